@@ -47,6 +47,13 @@ enum sk_status {
     SK_ERR_TIMEOUT = 6     /* a bounded device-side wait gave up               */
 };
 
+/* Element types of the operators that take more than float. */
+enum sk_dtype {
+    SK_FP32 = 0,
+    SK_BF16 = 1,
+    SK_FP16 = 2
+};
+
 /* Library version, major*10000 + minor*100 + patch. */
 int sk_version(void);
 
@@ -522,6 +529,53 @@ int sk_backward(const float* C, int64_t B, int64_t N, int64_t M, int64_t sCb,
                 const float* grad_f, const float* grad_g, float* dC, float* dlog_a,
                 float* dlog_b, void* workspace, size_t workspace_bytes, int* K,
                 void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Row distributions: log probabilities, entropy, best columns.            */
+
+/*
+ * For x_j = g_j + s X_ij (s = -1 when negate, else 1; X of type `dtype`, g
+ * fp32 (B,M) or NULL) and z = x / epsilon, per row i of each item:
+ *   lse      = log sum_j e^{z_j}
+ *   logprob  = z_t - lse at t = targets[i] (int64); 0 for t < 0 (none given),
+ *              NaN for t >= M
+ *   entropy  = -sum_j p_j log p_j
+ *   top_logprob, top_index: the top_k largest x_j (0 <= top_k <= min(32, M)),
+ *              equal ones by column; -inf and -1 where the row has fewer
+ *              columns above -inf
+ * Rows with mask_a = 0, and rows without a column above -inf, are empty:
+ * lse -inf, entropy 0, logprob -inf. mask_b = 0 leaves a column out, whatever
+ * X holds there. A NaN or +inf in a row makes its lse, logprob, entropy and
+ * top_logprob NaN. Any output may be NULL (logprob exactly when targets is;
+ * top_logprob and top_index only when top_k is 0). `stats` (2 floats per row)
+ * is what the backward needs. X may have any row strides; its columns have
+ * stride 1. The row form of the plan's conditional distribution
+ * (SinkhornOutput.transport_plan normalised by rows, src/sinkhorn/sinkhorn.py:27-54).
+ */
+int sk_row_logprobs(const void* X, int dtype, int64_t B, int64_t N, int64_t M, int64_t sXb,
+                    int64_t sXn, int64_t sXm, const float* g, double epsilon, int negate,
+                    const uint8_t* mask_a, const uint8_t* mask_b, const int64_t* targets,
+                    int top_k, float* lse, float* logprob, float* entropy, float* top_logprob,
+                    int64_t* top_index, float* stats, void* stream);
+
+/* Workspace bytes of sk_row_logprobs_backward (needed when dg is asked for). */
+size_t sk_row_logprobs_backward_workspace_bytes(int64_t B, int64_t N, int64_t M);
+
+/*
+ * Gradients of sk_row_logprobs: dX (dense (B,N,M), type of X) and dg (fp32
+ * (B,M)), either may be NULL. grad_* are fp32 and may be NULL each; `stats`,
+ * `entropy` and `top_index` are the forward's. Empty rows, targets that are
+ * not given, out of range or without probability and absent alternatives pass
+ * nothing. dg is summed over the rows in a fixed order.
+ */
+int sk_row_logprobs_backward(const void* X, int dtype, int64_t B, int64_t N, int64_t M,
+                             int64_t sXb, int64_t sXn, int64_t sXm, const float* g,
+                             double epsilon, int negate, const uint8_t* mask_b,
+                             const int64_t* targets, int top_k, const int64_t* top_index,
+                             const float* stats, const float* entropy, const float* grad_lse,
+                             const float* grad_logprob, const float* grad_entropy,
+                             const float* grad_top, void* dX, float* dg, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,9 @@ __version__ = "0.1.0"
 
 from .autograd import SinkhornFunction, sinkhorn_differentiable
 from .cuda.plan import marginal_error as compute_marginal_error
+from .logprobs import RowLogprobs, row_logprobs, token_logprobs
 from .sinkhorn import SinkhornOutput, sinkhorn
 
 __all__ = ["sinkhorn", "SinkhornOutput", "sinkhorn_differentiable", "SinkhornFunction",
-           "compute_marginal_error", "__version__"]
+           "compute_marginal_error", "RowLogprobs", "row_logprobs", "token_logprobs",
+           "__version__"]

@@ -105,6 +105,12 @@ SIGNATURES = {
     "sk_backward": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _D, _D,
                            _D, _INT, _D, _INT, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _IP,
                            _P]),
+    "sk_row_logprobs": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _D, _INT, _P,
+                               _P, _P, _INT, _P, _P, _P, _P, _P, _P, _P]),
+    "sk_row_logprobs_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "sk_row_logprobs_backward": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _D,
+                                        _INT, _P, _P, _INT, _P, _P, _P, _P, _P, _P, _P, _P,
+                                        _P, _P, _SZ, _P]),
 }
 
 _lock = threading.Lock()

@@ -69,6 +69,37 @@ def mask(x: Tensor | None, shape: tuple, device, name: str) -> Tensor | None:
     return (x != 0).contiguous().view(torch.uint8)
 
 
+# element types of the operators that take more than float32 (sk_dtype)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def check_cuda(x: Tensor, name: str) -> None:
+    if not isinstance(x, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} is on {x.device}: the cuda backend runs on CUDA tensors "
+                           "only (there is no CPU fallback)")
+
+
+def check_dtype(x: Tensor, name: str, allowed=tuple(DTYPES)) -> None:
+    if x.dtype not in allowed:
+        names = ", ".join(str(d).replace("torch.", "") for d in allowed)
+        raise TypeError(f"{name} must be one of {names}, got {x.dtype}")
+
+
+def indices(x: Tensor, shape: tuple, device, name: str) -> Tensor:
+    """A dense int64 tensor of `shape` on `device` from any integer type."""
+    if not isinstance(x, Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if x.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+        raise TypeError(f"{name} must hold integers, got {x.dtype}")
+    if tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, expected {device}")
+    return x.detach().to(torch.int64).contiguous()
+
+
 def workspace(nbytes: int, device) -> Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
 
