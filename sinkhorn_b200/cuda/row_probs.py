@@ -28,12 +28,16 @@ def row_probs(X: Tensor, g: Tensor | None, epsilon: float, negate: bool,
     top_lp = new(B, N, top_k) if top_k else None
     top_idx = new(B, N, top_k, dtype=torch.int64) if top_k else None
     if B * N:
+        lib = T.lib()
         with torch.cuda.device(dev):
-            rc = T.lib().sk_row_logprobs(
+            ws = None if mask_b is None else T.workspace(
+                lib.sk_row_logprobs_workspace_bytes(B, M), dev)
+            rc = lib.sk_row_logprobs(
                 X.data_ptr(), T.DTYPES[X.dtype], B, N, M, *X.stride(), T.ptr(g), epsilon,
                 int(negate), T.ptr(mask_a), T.ptr(mask_b), T.ptr(targets), top_k,
                 lse.data_ptr(), T.ptr(logprob), entropy.data_ptr(), T.ptr(top_lp),
-                T.ptr(top_idx), stats.data_ptr(), T.stream_of(dev))
+                T.ptr(top_idx), stats.data_ptr(), T.ptr(ws), 0 if ws is None else ws.numel(),
+                T.stream_of(dev))
             T.check(rc, "sk_row_logprobs")
     return lse, logprob, entropy, top_lp, top_idx, stats
 
@@ -61,7 +65,7 @@ def row_probs_backward(X: Tensor, g: Tensor | None, epsilon: float, negate: bool
     lib = T.lib()
     with torch.cuda.device(dev):
         ws = T.workspace(lib.sk_row_logprobs_backward_workspace_bytes(B, N, M), dev) \
-            if need_dg else None
+            if need_dg or mask_b is not None else None
         rc = lib.sk_row_logprobs_backward(
             X.data_ptr(), T.DTYPES[X.dtype], B, N, M, *X.stride(), T.ptr(g), epsilon,
             int(negate), T.ptr(mask_b), T.ptr(targets),
