@@ -556,9 +556,14 @@ int sk_row_logprobs(const void* X, int dtype, int64_t B, int64_t N, int64_t M, i
                     int64_t sXn, int64_t sXm, const float* g, double epsilon, int negate,
                     const uint8_t* mask_a, const uint8_t* mask_b, const int64_t* targets,
                     int top_k, float* lse, float* logprob, float* entropy, float* top_logprob,
-                    int64_t* top_index, float* stats, void* stream);
+                    int64_t* top_index, float* stats, void* workspace, size_t workspace_bytes,
+                    void* stream);
 
-/* Workspace bytes of sk_row_logprobs_backward (needed when dg is asked for). */
+/* Workspace bytes of sk_row_logprobs (needed with mask_b only). */
+size_t sk_row_logprobs_workspace_bytes(int64_t B, int64_t M);
+
+/* Workspace bytes of sk_row_logprobs_backward (needed with mask_b, and when dg
+ * is asked for). */
 size_t sk_row_logprobs_backward_workspace_bytes(int64_t B, int64_t N, int64_t M);
 
 /*
@@ -576,6 +581,51 @@ int sk_row_logprobs_backward(const void* X, int dtype, int64_t B, int64_t N, int
                              const float* grad_logprob, const float* grad_entropy,
                              const float* grad_top, void* dX, float* dg, void* workspace,
                              size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Experts: rows into the order of their experts and back.                 */
+
+size_t sk_expert_dispatch_workspace_bytes(int64_t slots, int experts);
+
+/*
+ * Stable counting sort of `slots` expert numbers (int64; those outside
+ * 0..experts-1 are dropped): offsets (experts+1) with offsets[0] = 0,
+ * position (slots): the place of each slot, -1 if dropped, order (slots): the
+ * slot at each place, -1 behind offsets[experts]. 1 <= experts <= 1024.
+ */
+int sk_expert_dispatch(const int64_t* index, int64_t slots, int experts, int* order,
+                       int* position, int* offsets, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/*
+ * rows[position[t,j]] = x[t] for the k slots of each of T tokens; rows (T k, D)
+ * dense, zero behind offsets[experts]. x has row stride ldx (elements) and
+ * unit column stride. A position outside 0..T k - 1 counts as dropped, here
+ * and below.
+ */
+int sk_dispatch_rows(const void* x, int dtype, int64_t T, int k, int64_t D, int64_t ldx,
+                     const int* position, const int* offsets, int experts, void* rows,
+                     void* stream);
+
+/*
+ * out[t] = sum_j weights[t,j] y[position[t,j]] in fp32, rounded once; weights
+ * (T,k) or NULL (all 1). out (T,D) dense. The adjoint of sk_dispatch_rows when
+ * weights is NULL.
+ */
+int sk_combine_rows(const void* y, int dtype, int64_t T, int k, int64_t D, int64_t ldy,
+                    const int* position, const int* offsets, int experts, const float* weights,
+                    void* out, void* stream);
+
+/*
+ * Gradients of sk_combine_rows: grad_y[position[t,j]] = weights[t,j]
+ * grad_out[t] (dense (T k, D), zero behind offsets[experts]) and
+ * grad_weights[t,j] = <grad_out[t], y[position[t,j]]> (0 where dropped).
+ * Either may be NULL.
+ */
+int sk_combine_rows_backward(const void* grad_out, const void* y, int dtype, int64_t T, int k,
+                             int64_t D, int64_t ldg, int64_t ldy, const int* position,
+                             const int* offsets, int experts, const float* weights, void* grad_y,
+                             float* grad_weights, void* stream);
 
 #ifdef __cplusplus
 }

@@ -106,11 +106,18 @@ SIGNATURES = {
                            _D, _INT, _D, _INT, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _IP,
                            _P]),
     "sk_row_logprobs": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _D, _INT, _P,
-                               _P, _P, _INT, _P, _P, _P, _P, _P, _P, _P]),
+                               _P, _P, _INT, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "sk_row_logprobs_workspace_bytes": (_SZ, [_I64, _I64]),
     "sk_row_logprobs_backward_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
     "sk_row_logprobs_backward": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _D,
                                         _INT, _P, _P, _INT, _P, _P, _P, _P, _P, _P, _P, _P,
                                         _P, _P, _SZ, _P]),
+    "sk_expert_dispatch_workspace_bytes": (_SZ, [_I64, _INT]),
+    "sk_expert_dispatch": (_INT, [_P, _I64, _INT, _P, _P, _P, _P, _SZ, _P]),
+    "sk_dispatch_rows": (_INT, [_P, _INT, _I64, _INT, _I64, _I64, _P, _P, _INT, _P, _P]),
+    "sk_combine_rows": (_INT, [_P, _INT, _I64, _INT, _I64, _I64, _P, _P, _INT, _P, _P, _P]),
+    "sk_combine_rows_backward": (_INT, [_P, _P, _INT, _I64, _INT, _I64, _I64, _I64, _P, _P,
+                                        _INT, _P, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

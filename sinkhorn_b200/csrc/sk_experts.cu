@@ -1,0 +1,522 @@
+// sk_experts.cu -- rows into the order of their experts and back.
+//
+// A router gives each token k experts (index, (T,k)). The S = T k slots are
+// put into expert order by a stable counting sort -- slot s = t k + j goes to
+//     position[s] = offsets[e] + #{s' < s : index[s'] = e},  e = index[s],
+// so the result does not depend on how the kernels are scheduled -- and the
+// tokens' rows are copied there (dispatch) and summed back with the gates'
+// weights (combine). Slots whose index is no expert are dropped; the rows
+// behind offsets[E] are zero.
+//
+// All three row kernels go by token, one warp each: the token's row is read or
+// written once, its k slots are whole rows elsewhere. They are bound by DRAM.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "sk_common.cuh"
+#include "sk_internal.h"
+
+namespace sk {
+namespace {
+
+constexpr int kSortThreads = 256;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortTile = 2048;  // slots of a CTA
+constexpr int kMaxExperts = 1024;
+
+__device__ __forceinline__ int expert_of(const int64_t* index, int64_t s, int64_t S, int E) {
+    if (s >= S) return -1;
+    const int64_t e = index[s];
+    return e >= 0 && e < E ? (int)e : -1;
+}
+
+// hist[tile][e]: the tile's slots of each expert.
+__global__ void __launch_bounds__(kSortThreads) k_expert_count(const int64_t* index, int64_t S,
+                                                              int E, int* hist) {
+    __shared__ int count[kMaxExperts];
+    for (int e = threadIdx.x; e < E; e += kSortThreads) count[e] = 0;
+    __syncthreads();
+    const int64_t s0 = (int64_t)blockIdx.x * kSortTile;
+#pragma unroll
+    for (int i = 0; i < kSortTile / kSortThreads; ++i) {
+        const int e = expert_of(index, s0 + i * kSortThreads + threadIdx.x, S, E);
+        if (e >= 0) atomicAdd(&count[e], 1);  // counts only: their order is no matter
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kSortThreads)
+        hist[(int64_t)blockIdx.x * E + e] = count[e];
+}
+
+// Places of the tile's slots. A warp takes a run of consecutive slots, 32 at a
+// time; lanes of one expert rank themselves by match.any.
+__global__ void __launch_bounds__(kSortThreads) k_expert_place(const int64_t* index, int64_t S,
+                                                              int E, int tiles, const int* hist,
+                                                              int* order, int* position,
+                                                              int* offsets) {
+    extern __shared__ int sm[];
+    int* const start = sm;      // [E] first place of the tile's slots of an expert
+    int* const wcount = sm + E;  // [warps][E]
+    __shared__ int wsum[kSortWarps];
+    __shared__ int carry;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t s0 =
+        (int64_t)blockIdx.x * kSortTile + warp * (kSortTile / kSortWarps);
+    constexpr int R = kSortTile / kSortThreads;
+    int e[R];
+    for (int i = threadIdx.x; i < kSortWarps * E; i += kSortThreads) wcount[i] = 0;
+    if (threadIdx.x == 0) carry = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) e[i] = expert_of(index, s0 + i * 32 + lane, S, E);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+        if (e[i] >= 0 && lane == __ffs(same) - 1) wcount[warp * E + e[i]] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    // Per expert: the earlier warps' counts, the earlier tiles', and the total,
+    // whose running sum over the experts gives the offsets.
+    for (int base = 0; base < E; base += kSortThreads) {
+        const int x = base + threadIdx.x;
+        int total = 0, before = 0;
+        if (x < E) {
+            int run = 0;
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) {
+                const int c = wcount[w * E + x];
+                wcount[w * E + x] = run;
+                run += c;
+            }
+            if (tiles == 1) {
+                total = run;
+            } else {
+#pragma unroll 8
+                for (int t = 0; t < tiles; ++t) {
+                    const int c = hist[(int64_t)t * E + x];
+                    if (t < (int)blockIdx.x) before += c;
+                    total += c;
+                }
+            }
+        }
+        int scan = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += v;
+        }
+        if (lane == 31) wsum[warp] = scan;
+        __syncthreads();
+        int add = carry;
+        for (int w = 0; w < warp; ++w) add += wsum[w];
+        if (x < E) {
+            start[x] = add + scan - total + before;
+            if (blockIdx.x == 0) offsets[x] = add + scan - total;
+        }
+        __syncthreads();
+        if (threadIdx.x == kSortThreads - 1) carry = add + scan;
+        __syncthreads();
+    }
+    const int held = carry;
+    if (blockIdx.x == 0 && threadIdx.x == 0) offsets[E] = held;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+        const int64_t s = s0 + i * 32 + lane;
+        int at = -1;
+        if (e[i] >= 0) {
+            at = start[e[i]] + wcount[warp * E + e[i]] + __popc(same & ((1u << lane) - 1u));
+            if (at < S) order[at] = (int)s;
+        }
+        if (s < S) position[s] = at;
+        __syncwarp();
+        if (e[i] >= 0 && lane == __ffs(same) - 1) wcount[warp * E + e[i]] += __popc(same);
+        __syncwarp();
+    }
+    // places behind the last group
+    for (int64_t p = held + (int64_t)blockIdx.x * kSortThreads + threadIdx.x; p < S;
+         p += (int64_t)gridDim.x * kSortThreads)
+        order[p] = -1;
+}
+
+// ------------------------------------------------------------------- rows
+
+// Words of W bytes: the widest that rows, strides and widths are multiples of.
+template <int W>
+struct WordOf;
+template <>
+struct WordOf<16> {
+    using type = uint4;
+};
+template <>
+struct WordOf<8> {
+    using type = uint2;
+};
+template <>
+struct WordOf<4> {
+    using type = uint32_t;
+};
+template <>
+struct WordOf<2> {
+    using type = uint16_t;
+};
+
+template <typename T, int W>
+struct Elems {
+    static constexpr int n = W / (int)sizeof(T);
+    union {
+        typename WordOf<W>::type word;
+        T e[n > 0 ? n : 1];
+    };
+    __device__ __forceinline__ Elems() {}
+    __device__ __forceinline__ float get(int i) const { return (float)e[i]; }
+    __device__ __forceinline__ void set(int i, float v) { e[i] = (T)v; }
+};
+
+struct RowsArgs {
+    const void *x, *y;  // rows by token (x) and by place (y)
+    void *ox, *oy;
+    int64_t ldx, ldy, ldox, ldoy;  // row strides in words
+    int64_t T;
+    int k;
+    int words;
+    const int* position;
+    const int* offsets;  // its last entry: rows that are held
+    int E;
+    const float* w;  // (T,k) or NULL
+    float* dw;       // (T,k)
+};
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 4;  // words of a row to a lane at once
+
+// The slot's place; one that is no row of the T k (a plan not made by
+// sk_expert_dispatch) counts as dropped.
+__device__ __forceinline__ int place_of(const RowsArgs& A, int64_t t, int j) {
+    const int p = __ldg(A.position + t * A.k + j);
+    return p < A.T * A.k ? p : -1;
+}
+
+template <int W>
+__device__ __forceinline__ void zero_rows_behind(const RowsArgs& A, int64_t gw, int64_t nw,
+                                                 int lane) {
+    using Word = typename WordOf<W>::type;
+    for (int64_t p = max(A.offsets[A.E], 0) + gw; p < A.T * A.k; p += nw) {
+        Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
+        for (int c = lane; c < A.words; c += 32) o[c] = Word{};
+    }
+}
+
+template <int W>
+__global__ void __launch_bounds__(kCopyThreads) k_dispatch_rows(const RowsArgs A) {
+    using Word = typename WordOf<W>::type;
+    const int lane = threadIdx.x & 31;
+    const int64_t gw = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) >> 5;
+    const int64_t nw = (int64_t)gridDim.x * (kCopyThreads / 32);
+    for (int64_t t = gw; t < A.T; t += nw) {
+        const Word* const x = reinterpret_cast<const Word*>(A.x) + t * A.ldx;
+        for (int c = lane; c < A.words; c += 32 * kCopyUnroll) {
+            Word v[kCopyUnroll];
+#pragma unroll
+            for (int u = 0; u < kCopyUnroll; ++u)
+                if (c + u * 32 < A.words) v[u] = x[c + u * 32];
+            for (int j = 0; j < A.k; ++j) {
+                const int p = place_of(A, t, j);
+                if (p < 0) continue;
+                Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
+#pragma unroll
+                for (int u = 0; u < kCopyUnroll; ++u)
+                    if (c + u * 32 < A.words) o[c + u * 32] = v[u];
+            }
+        }
+    }
+    zero_rows_behind<W>(A, gw, nw, lane);
+}
+
+// ox[t] = sum_j w[t,j] y[position[t,j]], in fp32, rounded once.
+template <typename T, int W>
+__global__ void __launch_bounds__(kCopyThreads) k_combine_rows(const RowsArgs A) {
+    using Word = typename WordOf<W>::type;
+    constexpr int n = W / (int)sizeof(T);
+    const int lane = threadIdx.x & 31;
+    const int64_t gw = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) >> 5;
+    const int64_t nw = (int64_t)gridDim.x * (kCopyThreads / 32);
+    for (int64_t t = gw; t < A.T; t += nw) {
+        Word* const o = reinterpret_cast<Word*>(A.ox) + t * A.ldox;
+        for (int c = lane; c < A.words; c += 32 * kCopyUnroll) {
+            float sum[kCopyUnroll][n];
+#pragma unroll
+            for (int u = 0; u < kCopyUnroll; ++u)
+#pragma unroll
+                for (int i = 0; i < n; ++i) sum[u][i] = 0.f;
+            for (int j = 0; j < A.k; ++j) {
+                const int p = place_of(A, t, j);
+                if (p < 0) continue;
+                const float w = A.w ? __ldg(A.w + t * A.k + j) : 1.f;
+                const Word* const y = reinterpret_cast<const Word*>(A.y) + p * A.ldy;
+                Elems<T, W> v[kCopyUnroll];
+#pragma unroll
+                for (int u = 0; u < kCopyUnroll; ++u)
+                    if (c + u * 32 < A.words) v[u].word = y[c + u * 32];
+#pragma unroll
+                for (int u = 0; u < kCopyUnroll; ++u)
+                    if (c + u * 32 < A.words)
+#pragma unroll
+                        for (int i = 0; i < n; ++i) sum[u][i] = fmaf(w, v[u].get(i), sum[u][i]);
+            }
+#pragma unroll
+            for (int u = 0; u < kCopyUnroll; ++u)
+                if (c + u * 32 < A.words) {
+                    Elems<T, W> v;
+#pragma unroll
+                    for (int i = 0; i < n; ++i) v.set(i, sum[u][i]);
+                    o[c + u * 32] = v.word;
+                }
+        }
+    }
+}
+
+// The adjoint of combine: with d = x[t] the upstream row of token t,
+//     oy[position[t,j]] = w[t,j] d,   dw[t,j] = <d, y[position[t,j]]>.
+// Either of oy and dw may be NULL.
+template <typename T, int W>
+__global__ void __launch_bounds__(kCopyThreads) k_combine_rows_bwd(const RowsArgs A) {
+    using Word = typename WordOf<W>::type;
+    constexpr int n = W / (int)sizeof(T);
+    const int lane = threadIdx.x & 31;
+    const int64_t gw = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) >> 5;
+    const int64_t nw = (int64_t)gridDim.x * (kCopyThreads / 32);
+    for (int64_t t = gw; t < A.T; t += nw) {
+        const Word* const x = reinterpret_cast<const Word*>(A.x) + t * A.ldx;
+        for (int j = 0; j < A.k; ++j) {
+            const int p = place_of(A, t, j);
+            float dot = 0.f;
+            if (p >= 0) {
+                const float w = A.w ? __ldg(A.w + t * A.k + j) : 1.f;
+                const Word* const y = reinterpret_cast<const Word*>(A.y) + p * A.ldy;
+                Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
+                for (int c = lane; c < A.words; c += 32 * kCopyUnroll) {
+                    Elems<T, W> d[kCopyUnroll], v[kCopyUnroll];
+#pragma unroll
+                    for (int u = 0; u < kCopyUnroll; ++u)
+                        if (c + u * 32 < A.words) {
+                            d[u].word = x[c + u * 32];
+                            if (A.dw) v[u].word = y[c + u * 32];
+                        }
+#pragma unroll
+                    for (int u = 0; u < kCopyUnroll; ++u)
+                        if (c + u * 32 < A.words) {
+                            if (A.dw)
+#pragma unroll
+                                for (int i = 0; i < n; ++i)
+                                    dot = fmaf(d[u].get(i), v[u].get(i), dot);
+                            if (A.oy) {
+#pragma unroll
+                                for (int i = 0; i < n; ++i) d[u].set(i, w * d[u].get(i));
+                                o[c + u * 32] = d[u].word;
+                            }
+                        }
+                }
+            }
+            if (A.dw) {
+                dot = warp_sum(dot);
+                if (lane == 0) A.dw[t * A.k + j] = dot;
+            }
+        }
+    }
+    if (A.oy) zero_rows_behind<W>(A, gw, nw, lane);
+}
+
+unsigned rows_grid(int64_t T) {
+    const int64_t ctas = (T + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(ctas, 148 * 64));
+}
+
+// The widest word (2 to 16 bytes) that every address, stride and width allows.
+int word_bytes(int64_t D, int elem, std::initializer_list<const void*> p,
+               std::initializer_list<int64_t> ld) {
+    int w = 16;
+    auto fit = [&](uint64_t v) {
+        while (v % w) w /= 2;
+    };
+    fit((uint64_t)D * elem);
+    for (const void* q : p) fit((uint64_t)(uintptr_t)q);
+    for (int64_t l : ld) fit((uint64_t)l * elem);
+    return w;
+}
+
+int check_rows_args(int dtype, int64_t T, int k, int64_t D, int E, const int* position,
+                    const int* offsets) {
+    if (dtype < SK_FP32 || dtype > SK_FP16) return fail(SK_ERR_ARG, "unknown element type");
+    if (T <= 0 || k <= 0 || D <= 0) return fail(SK_ERR_ARG, "T, k and D must be positive");
+    if (T > INT32_MAX / k || D > INT32_MAX / 4)
+        return fail(SK_ERR_ARG, "T * k must be below 2^31 and D below 2^29");
+    if (E <= 0 || E > kMaxExperts) return fail(SK_ERR_ARG, "experts must lie in 1..1024");
+    if (!position || !offsets) return fail(SK_ERR_ARG, "position or offsets is NULL");
+    return SK_OK;
+}
+
+template <int W>
+int run_dispatch(const RowsArgs& A, cudaStream_t s) {
+    k_dispatch_rows<W><<<rows_grid(A.T), kCopyThreads, 0, s>>>(A);
+    SK_LAUNCHED("k_dispatch_rows");
+    return SK_OK;
+}
+
+template <typename T, int W>
+int run_combine(const RowsArgs& A, bool bwd, cudaStream_t s) {
+    if (bwd) k_combine_rows_bwd<T, W><<<rows_grid(A.T), kCopyThreads, 0, s>>>(A);
+    else k_combine_rows<T, W><<<rows_grid(A.T), kCopyThreads, 0, s>>>(A);
+    SK_LAUNCHED(bwd ? "k_combine_rows_bwd" : "k_combine_rows");
+    return SK_OK;
+}
+
+template <typename T>
+int run_combine_wide(const RowsArgs& A, int w, bool bwd, cudaStream_t s) {
+    if (w == 16) return run_combine<T, 16>(A, bwd, s);
+    if (w == 8) return run_combine<T, 8>(A, bwd, s);
+    if constexpr (sizeof(T) == 2) {
+        if (w == 4) return run_combine<T, 4>(A, bwd, s);
+        return run_combine<T, 2>(A, bwd, s);
+    }
+    return run_combine<T, 4>(A, bwd, s);
+}
+
+int run_combine_typed(RowsArgs A, int dtype, int64_t D, bool bwd, cudaStream_t s) {
+    const int elem = dtype == SK_FP32 ? 4 : 2;
+    const int w = word_bytes(D, elem, {A.x, A.y, A.ox, A.oy}, {A.ldx, A.ldy, A.ldox, A.ldoy});
+    if (w < elem) return fail(SK_ERR_LAYOUT, "rows are not aligned to their elements");
+    const int per = w / elem;
+    A.words = (int)(D / per);
+    A.ldx /= per;
+    A.ldy /= per;
+    A.ldox /= per;
+    A.ldoy /= per;
+    if (dtype == SK_FP32) return run_combine_wide<float>(A, w, bwd, s);
+    if (dtype == SK_BF16) return run_combine_wide<__nv_bfloat16>(A, w, bwd, s);
+    return run_combine_wide<__half>(A, w, bwd, s);
+}
+
+int64_t sort_tiles(int64_t S) { return (S + kSortTile - 1) / kSortTile; }
+
+}  // namespace
+}  // namespace sk
+
+extern "C" {
+
+size_t sk_expert_dispatch_workspace_bytes(int64_t slots, int experts) {
+    if (slots <= 0 || experts <= 0) return 0;
+    return sk::align_up(sizeof(int) * (size_t)sk::sort_tiles(slots) * experts);
+}
+
+int sk_expert_dispatch(const int64_t* index, int64_t slots, int experts, int* order,
+                       int* position, int* offsets, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+    using namespace sk;
+    clear_error();
+    if (!index || !order || !position || !offsets)
+        return fail(SK_ERR_ARG, "index, order, position or offsets is NULL");
+    if (slots <= 0 || slots > INT32_MAX) return fail(SK_ERR_ARG, "slots must lie in 1..2^31-1");
+    if (experts <= 0 || experts > kMaxExperts)
+        return fail(SK_ERR_ARG, "experts must lie in 1..1024");
+    if (!workspace || workspace_bytes < sk_expert_dispatch_workspace_bytes(slots, experts))
+        return fail(SK_ERR_WORKSPACE, "workspace too small for sk_expert_dispatch");
+    cudaStream_t s = (cudaStream_t)stream;
+    const int tiles = (int)sort_tiles(slots);
+    if (tiles > 1) {
+        k_expert_count<<<tiles, kSortThreads, 0, s>>>(index, slots, experts, (int*)workspace);
+        SK_LAUNCHED("k_expert_count");
+    }
+    const size_t smem = sizeof(int) * (size_t)experts * (1 + kSortWarps);
+    k_expert_place<<<tiles, kSortThreads, smem, s>>>(index, slots, experts, tiles,
+                                                     (const int*)workspace, order, position,
+                                                     offsets);
+    SK_LAUNCHED("k_expert_place");
+    return SK_OK;
+}
+
+int sk_dispatch_rows(const void* x, int dtype, int64_t T, int k, int64_t D, int64_t ldx,
+                     const int* position, const int* offsets, int experts, void* rows,
+                     void* stream) {
+    using namespace sk;
+    clear_error();
+    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
+    if (rc != SK_OK) return rc;
+    if (!x || !rows) return fail(SK_ERR_ARG, "x or rows is NULL");
+    if (ldx < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
+    const int elem = dtype == SK_FP32 ? 4 : 2;
+    const int w = word_bytes(D, elem, {x, rows}, {ldx, D});
+    if (w < elem) return fail(SK_ERR_LAYOUT, "rows are not aligned to their elements");
+    RowsArgs A{};
+    A.x = x;
+    A.oy = rows;
+    A.ldx = ldx * elem / w;
+    A.ldoy = D * elem / w;
+    A.T = T;
+    A.k = k;
+    A.words = (int)(D * elem / w);
+    A.position = position;
+    A.offsets = offsets;
+    A.E = experts;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (w == 16) return run_dispatch<16>(A, s);
+    if (w == 8) return run_dispatch<8>(A, s);
+    if (w == 4) return run_dispatch<4>(A, s);
+    return run_dispatch<2>(A, s);
+}
+
+int sk_combine_rows(const void* y, int dtype, int64_t T, int k, int64_t D, int64_t ldy,
+                    const int* position, const int* offsets, int experts, const float* weights,
+                    void* out, void* stream) {
+    using namespace sk;
+    clear_error();
+    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
+    if (rc != SK_OK) return rc;
+    if (!y || !out) return fail(SK_ERR_ARG, "y or out is NULL");
+    if (ldy < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
+    RowsArgs A{};
+    A.y = y;
+    A.ox = out;
+    A.ldy = ldy;
+    A.ldox = D;
+    A.T = T;
+    A.k = k;
+    A.position = position;
+    A.offsets = offsets;
+    A.E = experts;
+    A.w = weights;
+    return run_combine_typed(A, dtype, D, false, (cudaStream_t)stream);
+}
+
+int sk_combine_rows_backward(const void* grad_out, const void* y, int dtype, int64_t T, int k,
+                             int64_t D, int64_t ldg, int64_t ldy, const int* position,
+                             const int* offsets, int experts, const float* weights, void* grad_y,
+                             float* grad_weights, void* stream) {
+    using namespace sk;
+    clear_error();
+    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
+    if (rc != SK_OK) return rc;
+    if (!grad_out) return fail(SK_ERR_ARG, "grad_out is NULL");
+    if (!grad_y && !grad_weights) return fail(SK_ERR_ARG, "no gradient is asked for");
+    if (grad_weights && !y) return fail(SK_ERR_ARG, "grad_weights needs y");
+    if (ldg < 0 || ldy < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
+    RowsArgs A{};
+    A.x = grad_out;
+    A.y = y;
+    A.oy = grad_y;
+    A.ldx = ldg;
+    A.ldy = ldy;
+    A.ldoy = D;
+    A.T = T;
+    A.k = k;
+    A.position = position;
+    A.offsets = offsets;
+    A.E = experts;
+    A.w = weights;
+    A.dw = grad_weights;
+    return run_combine_typed(A, dtype, D, true, (cudaStream_t)stream);
+}
+
+}  // extern "C"

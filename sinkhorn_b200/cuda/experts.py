@@ -1,0 +1,91 @@
+"""Rows into the order of their experts and back (C ABI wrappers): the stable
+sort of a router's choices, the copy of token rows into it, their weighted sum
+and its adjoint. ``sinkhorn_b200.experts`` is the differentiable front end.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from .. import _tensors as T
+
+
+def sort_slots(index: Tensor, n_experts: int) -> tuple[Tensor, Tensor, Tensor]:
+    """sk_expert_dispatch on a dense int64 index (T, k): (order, position, offsets)."""
+    dev, slots = index.device, index.numel()
+    order = torch.empty(slots, device=dev, dtype=torch.int32)
+    position = torch.empty(index.shape, device=dev, dtype=torch.int32)
+    if not slots:
+        return order, position, torch.zeros(n_experts + 1, device=dev, dtype=torch.int32)
+    offsets = torch.empty(n_experts + 1, device=dev, dtype=torch.int32)
+    lib = T.lib()
+    with torch.cuda.device(dev):
+        ws = T.workspace(lib.sk_expert_dispatch_workspace_bytes(slots, n_experts), dev)
+        rc = lib.sk_expert_dispatch(index.data_ptr(), slots, n_experts, order.data_ptr(),
+                                    position.data_ptr(), offsets.data_ptr(), ws.data_ptr(),
+                                    ws.numel(), T.stream_of(dev))
+        T.check(rc, "sk_expert_dispatch")
+    return order, position, offsets
+
+
+def unit_rows(x: Tensor) -> Tensor:
+    """x itself where its columns have unit stride, else a dense copy."""
+    return x if x.stride(1) == 1 or x.shape[1] == 1 and x.is_contiguous() else x.contiguous()
+
+
+def gather_rows(x: Tensor, position: Tensor, offsets: Tensor) -> Tensor:
+    """sk_dispatch_rows: rows (T k, D) of x (T, D)."""
+    x = unit_rows(x)
+    t, k = position.shape
+    D = x.shape[1]
+    rows = torch.empty(t * k, D, device=x.device, dtype=x.dtype)
+    if rows.numel():
+        with torch.cuda.device(x.device):
+            rc = T.lib().sk_dispatch_rows(
+                x.data_ptr(), T.DTYPES[x.dtype], t, k, D, x.stride(0), position.data_ptr(),
+                offsets.data_ptr(), offsets.numel() - 1, rows.data_ptr(),
+                T.stream_of(x.device))
+            T.check(rc, "sk_dispatch_rows")
+    return rows
+
+
+def sum_rows(y: Tensor, position: Tensor, offsets: Tensor, weights: Tensor | None) -> Tensor:
+    """sk_combine_rows: (T, D) from y (T k, D); weights dense float32 (T, k) or None."""
+    y = unit_rows(y)
+    t, k = position.shape
+    D = y.shape[1]
+    out = torch.empty(t, D, device=y.device, dtype=y.dtype)
+    if not out.numel():
+        return out
+    if not k:
+        return out.zero_()
+    with torch.cuda.device(y.device):
+        rc = T.lib().sk_combine_rows(
+            y.data_ptr(), T.DTYPES[y.dtype], t, k, D, y.stride(0), position.data_ptr(),
+            offsets.data_ptr(), offsets.numel() - 1, T.ptr(weights), out.data_ptr(),
+            T.stream_of(y.device))
+        T.check(rc, "sk_combine_rows")
+    return out
+
+
+def sum_rows_backward(grad: Tensor, y: Tensor, position: Tensor, offsets: Tensor,
+                      weights: Tensor | None, need_y: bool, need_w: bool):
+    """sk_combine_rows_backward: (grad_y, grad_weights); unneeded ones are None."""
+    t, k = position.shape
+    D = y.shape[1]
+    grad = unit_rows(grad)
+    y = unit_rows(y)
+    dy = torch.empty(t * k, D, device=y.device, dtype=y.dtype) if need_y else None
+    dw = torch.empty(t, k, device=y.device, dtype=torch.float32) if need_w else None
+    if not t * k or not (need_y or need_w):
+        return dy, dw
+    if not D:
+        return dy, None if dw is None else dw.zero_()
+    with torch.cuda.device(y.device):
+        rc = T.lib().sk_combine_rows_backward(
+            grad.data_ptr(), y.data_ptr(), T.DTYPES[y.dtype], t, k, D, grad.stride(0),
+            y.stride(0), position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
+            T.ptr(weights), T.ptr(dy), T.ptr(dw), T.stream_of(y.device))
+        T.check(rc, "sk_combine_rows_backward")
+    return dy, dw
