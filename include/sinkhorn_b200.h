@@ -627,6 +627,37 @@ int sk_combine_rows_backward(const void* grad_out, const void* y, int dtype, int
                              const int* offsets, int experts, const float* weights, void* grad_y,
                              float* grad_weights, void* stream);
 
+/* Workspace bytes of sk_grouped_matmul: 0 when x and w start every row on 16
+ * bytes (only the addresses' alignment is looked at). */
+size_t sk_grouped_matmul_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
+                                         const void* w, int64_t E, int64_t N, int64_t swe,
+                                         int64_t swk, int64_t swn);
+
+/*
+ * y[r] = x[r] W_e for the rows r of group e, offsets[e] <= r < offsets[e+1];
+ * rows of no group are zero. x (S,K) with row stride ldx, W (E,K,N) with
+ * element strides swe, swk, swn (swk or swn is 1), y (S,N) dense; all bf16 or
+ * all fp16, sums in fp32, rounded once. offsets (E+1) is device memory;
+ * entries that fall or leave [0,S] are brought back. E <= 1024. The gradient
+ * of x is the same call on dy with K, N and swk, swn exchanged.
+ */
+int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ldx, const void* w,
+                      int64_t E, int64_t N, int64_t swe, int64_t swk, int64_t swn,
+                      const int* offsets, void* y, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+size_t sk_grouped_matmul_weight_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
+                                                const void* dy, int64_t N, int64_t ldy);
+
+/*
+ * dW_e = sum over the rows r of group e of x[r]^T dy[r]: (E,K,N) dense, or
+ * (E,N,K) dense when `transposed`; zero for a group without rows.
+ */
+int sk_grouped_matmul_weight(const void* x, int dtype, int64_t S, int64_t K, int64_t ldx,
+                             const void* dy, int64_t N, int64_t ldy, const int* offsets,
+                             int64_t E, void* dw, int transposed, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

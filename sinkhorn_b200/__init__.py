@@ -10,11 +10,13 @@ __version__ = "0.1.0"
 
 from .autograd import SinkhornFunction, sinkhorn_differentiable
 from .cuda.plan import marginal_error as compute_marginal_error
-from .experts import ExpertDispatch, combine_rows, dispatch_rows, expert_dispatch
+from .experts import (ExpertDispatch, combine_rows, dispatch_rows, expert_dispatch,
+                      grouped_matmul)
 from .logprobs import RowLogprobs, row_logprobs, token_logprobs
 from .sinkhorn import SinkhornOutput, sinkhorn
 
 __all__ = ["sinkhorn", "SinkhornOutput", "sinkhorn_differentiable", "SinkhornFunction",
            "compute_marginal_error", "RowLogprobs", "row_logprobs", "token_logprobs",
            "ExpertDispatch", "expert_dispatch", "dispatch_rows", "combine_rows",
+           "grouped_matmul",
            "__version__"]

@@ -1,6 +1,6 @@
 """Rows into the order of their experts and back (C ABI wrappers): the stable
 sort of a router's choices, the copy of token rows into it, their weighted sum
-and its adjoint. ``sinkhorn_b200.experts`` is the differentiable front end.
+and its adjoint; and the experts' products over ragged runs of rows. ``sinkhorn_b200.experts`` is the differentiable front end.
 """
 
 from __future__ import annotations
@@ -89,3 +89,57 @@ def sum_rows_backward(grad: Tensor, y: Tensor, position: Tensor, offsets: Tensor
             T.ptr(weights), T.ptr(dy), T.ptr(dw), T.stream_of(y.device))
         T.check(rc, "sk_combine_rows_backward")
     return dy, dw
+
+
+def _weight_strides(w: Tensor) -> tuple[int, int, int]:
+    """Strides of w (E, K, N); an axis of one element has stride 1."""
+    return tuple(s if n > 1 else 1 for s, n in zip(w.stride(), w.shape))
+
+
+def unit_weights(w: Tensor) -> Tensor:
+    """w itself where one of its last two axes has unit stride, else a dense copy."""
+    _, sk, sn = _weight_strides(w)
+    return w if sk == 1 or sn == 1 else w.contiguous()
+
+
+def product(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
+    """sk_grouped_matmul: (S, N) from x (S, K), w (E, K, N) (unit_weights) and offsets."""
+    x = unit_rows(x)
+    S, K = x.shape
+    E, _, N = w.shape
+    y = torch.empty(S, N, device=x.device, dtype=x.dtype)
+    if not y.numel():
+        return y
+    if not K:
+        return y.zero_()
+    lib = T.lib()
+    with torch.cuda.device(x.device):
+        args = (S, K, x.stride(0), w.data_ptr(), E, N, *_weight_strides(w))
+        n = lib.sk_grouped_matmul_workspace_bytes(x.data_ptr(), *args)
+        ws = T.workspace(n, x.device) if n else None
+        rc = lib.sk_grouped_matmul(x.data_ptr(), T.DTYPES[x.dtype], *args, offsets.data_ptr(),
+                                   y.data_ptr(), T.ptr(ws), n, T.stream_of(x.device))
+        T.check(rc, "sk_grouped_matmul")
+    return y
+
+
+def weight_product(x: Tensor, dy: Tensor, offsets: Tensor, transposed: bool) -> Tensor:
+    """sk_grouped_matmul_weight: dW (E, K, N), laid out (E, N, K) when ``transposed``."""
+    x, dy = unit_rows(x), unit_rows(dy)
+    S, K = x.shape
+    N, E = dy.shape[1], offsets.numel() - 1
+    dw = torch.empty((E, N, K) if transposed else (E, K, N), device=x.device, dtype=x.dtype)
+    if not S:
+        dw.zero_()
+    elif dw.numel():
+        lib = T.lib()
+        with torch.cuda.device(x.device):
+            n = lib.sk_grouped_matmul_weight_workspace_bytes(
+                x.data_ptr(), S, K, x.stride(0), dy.data_ptr(), N, dy.stride(0))
+            ws = T.workspace(n, x.device) if n else None
+            rc = lib.sk_grouped_matmul_weight(
+                x.data_ptr(), T.DTYPES[x.dtype], S, K, x.stride(0), dy.data_ptr(), N,
+                dy.stride(0), offsets.data_ptr(), E, dw.data_ptr(), int(transposed),
+                T.ptr(ws), n, T.stream_of(x.device))
+            T.check(rc, "sk_grouped_matmul_weight")
+    return dw.transpose(1, 2) if transposed else dw

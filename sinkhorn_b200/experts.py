@@ -2,9 +2,10 @@
 
 A router (a transport plan's best columns, ``row_logprobs(..., top_k=k)``) gives each
 token k experts. ``expert_dispatch`` sorts these choices by expert, ``dispatch_rows``
-copies the tokens' rows into that order, so that each expert's rows are consecutive, and
-``combine_rows`` sums each token's k results with its gates. All but the sort are
-differentiable; nothing here synchronises with the host.
+copies the tokens' rows into that order, so that each expert's rows are consecutive,
+``grouped_matmul`` multiplies them by their experts' weights, and ``combine_rows`` sums each
+token's k results with its gates. All but the sort are differentiable; nothing here
+synchronises with the host.
 """
 
 from __future__ import annotations
@@ -17,7 +18,8 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _tensors as T
-from .cuda.experts import gather_rows, sort_slots, sum_rows, sum_rows_backward
+from .cuda.experts import (gather_rows, product, sort_slots, sum_rows, sum_rows_backward,
+                           unit_weights, weight_product)
 
 MAX_EXPERTS = 1024
 
@@ -152,3 +154,58 @@ def combine_rows(y: Tensor, dispatch: ExpertDispatch, weights: Tensor | None = N
         if weights.device != y.device:
             raise ValueError(f"weights are on {weights.device}, y is on {y.device}")
     return CombineRowsFunction.apply(y, weights, dispatch.position, dispatch.offsets)
+
+
+class GroupedMatmulFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
+        ctx.save_for_backward(x, w, offsets)
+        return product(x.detach(), w.detach(), offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad: Tensor):
+        x, w, offsets = ctx.saved_tensors
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = product(grad, w.detach().transpose(1, 2), offsets)
+        if ctx.needs_input_grad[1]:
+            dw = weight_product(x.detach(), grad, offsets, transposed=w.stride(2) != 1)
+        return dx, dw, None
+
+
+def grouped_matmul(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
+    """``y[r] = x[r] @ w[e]`` for the rows r of each group e: (S, N).
+
+    x (S, K) and w (E, K, N), both bfloat16 or both float16; offsets (E + 1,) int32 or
+    int64 on the device, group e holds rows ``offsets[e]`` to ``offsets[e + 1] - 1`` (as
+    ``expert_dispatch`` gives them). Groups may be empty; rows of no group give zeros and
+    get zero gradient. Offsets that decrease or leave 0..S are clamped. Sums are in fp32,
+    rounded once. Any K and N; rows that do not start on 16 bytes (K or N no multiple of 8)
+    are copied once more. w may be stored (E, N, K) and passed transposed; its gradient then
+    has that layout, too. Up to 1024 groups.
+    """
+    for name, t, dims in (("x", x, 2), ("w", w, 3)):
+        T.check_cuda(t, name)
+        if t.dim() != dims:
+            raise ValueError(f"{name} must be {dims}D, got {t.dim()}D")
+        T.check_dtype(t, name, (torch.bfloat16, torch.float16))
+    if x.dtype != w.dtype:
+        raise TypeError(f"x is {x.dtype}, w is {w.dtype}: they must have one type")
+    if w.device != x.device:
+        raise ValueError(f"w is on {w.device}, x is on {x.device}")
+    E, K, _ = w.shape
+    if x.shape[1] != K:
+        raise ValueError(f"x has {x.shape[1]} columns, w has {K} rows")
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"w must hold 1 to {MAX_EXPERTS} groups, got {E}")
+    if not isinstance(offsets, Tensor):
+        raise TypeError("offsets must be a torch.Tensor")
+    if offsets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"offsets must be int32 or int64, got {offsets.dtype}")
+    if tuple(offsets.shape) != (E + 1,):
+        raise ValueError(f"offsets must have shape {(E + 1,)}, got {tuple(offsets.shape)}")
+    if offsets.device != x.device:
+        raise ValueError(f"offsets are on {offsets.device}, x is on {x.device}")
+    offsets = offsets.detach().to(torch.int32).contiguous()
+    return GroupedMatmulFunction.apply(x, unit_weights(w), offsets)
