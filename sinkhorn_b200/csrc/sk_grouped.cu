@@ -8,10 +8,17 @@
 // One tensor-core kernel does both. A tile of the output is computed as
 //     D[m, c] = sum_k A[m, k] B[c, k],   out[c * ldo + m] = D[m, c],
 // with m the output's contiguous dimension on the 128 lanes of tensor memory and
-// c, of any multiple of 16 up to 256, on its columns. For `rows` c is the ragged
+// c, of any multiple of 32 up to 256, on its columns. For `rows` c is the ragged
 // dimension: the instruction's N is chosen per tile, so a group of r rows costs
-// ceil(r / 16) * 16 columns and not whole tiles, and the weights are the operand
-// that is always full. For `weights` the last block of a run's contraction holds
+// ceil(r / 32) * 32 columns and not whole tiles, and the weights are the operand
+// that is always full.
+//
+// Two CTAs work on a tile of 256 lanes (cta_group::2): each brings its own 128
+// lanes of A and half of the columns of B. Alone, a CTA would read 12 KB of
+// shared memory for each 128 x 256 x 16 product and write as much, 192 cycles
+// at 128 bytes for 128 cycles of products; the pair needs 8 KB and 8 KB.
+//
+// For `weights` the last block of a run's contraction holds
 // rows of the next group; they are cleared in shared memory before they are used
 // (a zero in one operand alone would not do: 0 * inf).
 #include <cudaTypedefs.h>
@@ -20,23 +27,33 @@
 
 #include <algorithm>
 
+#include "sk_cluster.cuh"
 #include "sk_internal.h"
 #include "sk_tcgen05.cuh"
 
 namespace sk {
 namespace {
 
-constexpr int kBM = 128;    // lanes: the output's contiguous dimension
-constexpr int kBN = 256;    // most columns of a tile
-constexpr int kBK = 64;     // contraction of a stage: one 128-byte swizzled row
-constexpr int kStages = 4;
+constexpr int kBM = 128;     // lanes of a CTA: the output's contiguous dimension
+constexpr int kPairM = 256;  // of the two
+constexpr int kBK = 64;      // contraction of a stage: one 128-byte swizzled row
 constexpr int kABytes = kBM * kBK * 2;
-constexpr int kBBytes = kBN * kBK * 2;
-constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kBandC = 8;   // column tiles that share a pass over the weights
+constexpr int kBox = 64 * kBK * 2;  // bytes of 64 x 64 elements
+constexpr int kBandC = 8;    // column tiles that share a pass over the weights
 constexpr int kThreads = 192;  // producer warp, MMA warp, four epilogue warps
 constexpr int kMaxGroups = 1024;
-constexpr uint32_t kTmemCols = 512;  // two accumulators
+
+// BN: most columns of a tile. 256, or 64 for short groups, whose products are
+// bound by the read of the weights: a stage is then nearly all weights and more
+// of them are in flight.
+template <int BN>
+struct Shape {
+    static constexpr int kHalf = BN / 2;  // columns of B in each CTA
+    static constexpr int kStageBytes = kABytes + kHalf * kBK * 2;
+    static constexpr int kStages = BN == 256 ? 6 : 10;
+    static constexpr uint32_t kTmemCols = 2 * BN;  // two accumulators
+};
+constexpr int kMaxStages = 10;
 
 struct GroupedArgs {
     CUtensorMap a, b, b32;  // b32: boxes of 32 columns, for narrow tiles
@@ -49,7 +66,12 @@ struct GroupedArgs {
 };
 
 struct alignas(8) GroupedShared {
-    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+    // full (the leading CTA's): the copies of both CTAs of a stage have landed.
+    // empty, acc_full: committed by the MMAs to both. A stage whose last rows are
+    // cleared takes another way: the second CTA's copies complete on its own
+    // `part`, and it signals the leading CTA's `ready` once they are cleared.
+    uint64_t full[kMaxStages], empty[kMaxStages], part[kMaxStages], ready[kMaxStages];
+    uint64_t acc_full[2], acc_empty[2], drain;
     uint32_t tmem;
     int gave_up;  // a bounded wait ran out: the CTA's remaining tiles become NaN
     int tiles;
@@ -66,22 +88,37 @@ struct Tile {
     int k0, depth;  // contraction: first index, extent
 };
 
-__device__ __forceinline__ bool wait_or_give_up(GroupedShared* sh, uint64_t* bar,
-                                                uint32_t parity) {
-    for (uint32_t i = 0; i < kWaitPolls; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*reinterpret_cast<volatile int*>(&sh->gave_up)) return false;
-    }
-    *reinterpret_cast<volatile int*>(&sh->gave_up) = 1;
-    return false;
+// A wait that ran out (or saw another run out) marks the CTA.
+__device__ __forceinline__ bool flagged(GroupedShared* sh, bool ok) {
+    if (!ok) *reinterpret_cast<volatile int*>(&sh->gave_up) = 1;
+    return ok;
+}
+__device__ __forceinline__ bool wait_local(GroupedShared* sh, uint64_t* bar, uint32_t parity) {
+    return flagged(sh, wait_full(bar, parity, &sh->gave_up));
+}
+// One lane polls for the warp: 32 would take the barrier unit's time from the
+// copies and commits that complete there.
+__device__ __forceinline__ bool wait_local_warp(GroupedShared* sh, uint64_t* bar, uint32_t parity,
+                                                int lane) {
+    const bool ok = lane != 0 || wait_local(sh, bar, parity);
+    return __shfl_sync(0xffffffffu, (int)ok, 0);
+}
+__device__ __forceinline__ bool wait_peer_warp(GroupedShared* sh, uint64_t* bar, uint32_t parity,
+                                               int lane) {
+    const bool ok = lane != 0 || flagged(sh, wait_peer(bar, parity, &sh->gave_up));
+    return __shfl_sync(0xffffffffu, (int)ok, 0);
 }
 
-__device__ __forceinline__ int column_tiles(int rows) { return (rows + kBN - 1) / kBN; }
+template <int BN>
+__device__ __forceinline__ int column_tiles(int rows) {
+    return (rows + BN - 1) / BN;
+}
 
 // Tile t of the launch.
+template <int BN>
 __device__ __forceinline__ Tile tile_at(const GroupedArgs& A, const GroupedShared* sh, int t) {
     Tile q;
-    const int nm = (A.m + kBM - 1) / kBM;
+    const int nm = (A.m + kPairM - 1) / kPairM;
     if (A.by_rows) {
         int lo = 0, hi = A.E + 1;  // the last group whose first tile is <= t
         while (lo < hi) {
@@ -90,30 +127,30 @@ __device__ __forceinline__ Tile tile_at(const GroupedArgs& A, const GroupedShare
             else hi = mid - 1;
         }
         const int r0 = sh->first[lo], rows = sh->first[lo + 1] - r0;
-        const int nc = column_tiles(rows);
+        const int nc = column_tiles<BN>(rows);
         // even tiles, in bands that reuse what of the weights they have loaded
-        const int each = ((rows + nc - 1) / nc + 15) / 16 * 16;
+        const int each = ((rows + nc - 1) / nc + 31) / 32 * 32;
         int l = t - sh->tile0[lo];
         const int band = l / (kBandC * nm);
         l -= band * kBandC * nm;
         const int wide = min(kBandC, nc - band * kBandC);
         const int c = band * kBandC + l % wide;
         q.group = lo >= 1 && lo <= A.E ? lo - 1 : -1;
-        q.m0 = l / wide * kBM;
+        q.m0 = l / wide * kPairM;
         q.c0 = r0 + c * each;
         q.cols = min(each, rows - c * each);
         q.k0 = 0;
         q.depth = q.group >= 0 ? A.k : 0;
     } else {
-        const int nc = column_tiles(A.c);
+        const int nc = column_tiles<BN>(A.c);
         q.group = t / (nm * nc);
         int l = t - q.group * nm * nc;
         const int band = l / (kBandC * nm);
         l -= band * kBandC * nm;
         const int wide = min(kBandC, nc - band * kBandC);
-        q.m0 = l / wide * kBM;
-        q.c0 = (band * kBandC + l % wide) * kBN;
-        q.cols = min(kBN, A.c - q.c0);
+        q.m0 = l / wide * kPairM;
+        q.c0 = (band * kBandC + l % wide) * BN;
+        q.cols = min(BN, A.c - q.c0);
         q.k0 = sh->first[q.group + 1];
         q.depth = sh->first[q.group + 2] - q.k0;
     }
@@ -135,8 +172,9 @@ __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
 
 // Group bounds and tile counts, by one warp. Offsets that fall or leave [0, S]
 // are brought back: no tile then reaches outside the rows.
+template <int BN>
 __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
-    const int nm = (A.m + kBM - 1) / kBM;
+    const int nm = (A.m + kPairM - 1) / kPairM;
     int reach = 0, tiles = 0;  // running maximum of the offsets, running tile count
     if (lane == 0) sh->first[0] = 0;
     for (int base = 0; base <= A.E + 1; base += 32) {
@@ -151,7 +189,7 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
         o = max(o, reach);
         int before = __shfl_up_sync(0xffffffffu, o, 1);
         if (lane == 0) before = reach;
-        int n = i <= A.E + 1 ? column_tiles(o - before) * nm : 0;  // tiles of group i
+        int n = i <= A.E + 1 ? column_tiles<BN>(o - before) * nm : 0;  // tiles of group i
         int sum = n;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
@@ -165,22 +203,24 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
         reach = __shfl_sync(0xffffffffu, o, 31);
         tiles += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) sh->tiles = A.by_rows ? tiles : A.E * nm * column_tiles(A.c);
+    if (lane == 0) sh->tiles = A.by_rows ? tiles : A.E * nm * column_tiles<BN>(A.c);
 }
 
-template <typename T>
-__device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh, int quarter,
-                                         int lane) {
+template <typename T, int BN>
+__device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh, int rank,
+                                         int quarter, int lane) {
     int used = 0;  // accumulators so far
-    for (int t = blockIdx.x; t < sh->tiles; t += gridDim.x) {
-        const Tile q = tile_at(A, sh, t);
+    const uint32_t release0 = map_to_rank(&sh->acc_empty[0], 0);
+    const uint32_t release1 = map_to_rank(&sh->acc_empty[1], 0);
+    for (int t = blockIdx.x / 2; t < sh->tiles; t += gridDim.x / 2) {
+        const Tile q = tile_at<BN>(A, sh, t);
         T* const out = reinterpret_cast<T*>(A.out) +
                        (A.by_rows ? 0 : q.group * A.out_group) + (int64_t)q.c0 * A.ldo;
-        const int m = q.m0 + quarter * 32 + lane;
+        const int m = q.m0 + rank * kBM + quarter * 32 + lane;
         const int buf = used & 1;
         bool ok = true;
         if (q.depth > 0) {
-            ok = wait_or_give_up(sh, &sh->acc_full[buf], (used >> 1) & 1);
+            ok = wait_local_warp(sh, &sh->acc_full[buf], (used >> 1) & 1, lane);
             tc_fence_after();
         }
         // pairs of lanes exchange so that each stores two neighbours of a column
@@ -188,7 +228,7 @@ __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh
         for (int c = 0; c < q.cols; c += 32) {
             uint32_t v[32];
             if (q.depth > 0 && ok) {
-                tmem_ld32(sh->tmem + ((uint32_t)(quarter * 32) << 16) + buf * kBN + c, v);
+                tmem_ld32(sh->tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + c, v);
                 tmem_ld_wait();
             } else {
                 const float fill = ok ? 0.f : NAN;
@@ -221,31 +261,75 @@ __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh
         if (q.depth > 0) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->acc_empty[buf]);
+            if (lane == 0) mbar_signal_cluster(buf ? release1 : release0);
             ++used;
         }
     }
 }
 
+// A place in the ring of stages: the stage, and how often the ring went round.
+template <int N>
+struct Ring {
+    int s = 0;
+    uint32_t lap = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == N) {
+            s = 0;
+            ++lap;
+        }
+    }
+    __device__ __forceinline__ void skip(int n) {
+        s += n;
+        lap += s / N;
+        s %= N;
+    }
+};
+
+// Rows behind the contraction that the last of its 16-deep steps reads: of the
+// next group where the rows are the contraction (else the copy engine's zeros).
+__device__ __forceinline__ int cleared_rows(const GroupedArgs& A, int left) {
+    return A.by_rows || left >= kBK ? 0 : (left + 15) / 16 * 16 - left;
+}
+
+// Clear them in a stage of MN-major operands, by one warp: a row is 128 bytes of
+// each box of 64 columns, whatever the swizzle.
+__device__ __forceinline__ void clear_rows(uint8_t* stage, int n, int left, int rows, int lane) {
+    const int boxes = 2 + (n / 2 + 63) / 64;
+    for (int i = lane; i < boxes * rows * 8; i += 32) {
+        const int x = i / (rows * 8), r = i / 8 % rows;
+        *reinterpret_cast<uint4*>(stage + x * kBox + (left + r) * 128 + i % 8 * 16) =
+            make_uint4(0, 0, 0, 0);
+    }
+    fence_async_smem();
+    __syncwarp();
+}
+
+template <int BN>
 __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__ GroupedArgs A) {
+    using Z = Shape<BN>;
     extern __shared__ uint8_t dyn[];
     uint8_t* const stages =
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    GroupedShared* const sh = reinterpret_cast<GroupedShared*>(stages + kStages * kStageBytes);
+    GroupedShared* const sh =
+        reinterpret_cast<GroupedShared*>(stages + Z::kStages * Z::kStageBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    const int t0 = blockIdx.x / 2, dt = gridDim.x / 2;  // the pair's tiles
 
     if (warp == 0) {
-        plan_groups(A, sh, lane);
+        plan_groups<BN>(A, sh, lane);
     } else if (warp == 1) {
-        tmem_alloc(&sh->tmem, kTmemCols);
+        tmem_alloc_pair(&sh->tmem, Z::kTmemCols);
         if (lane == 0) {
-            for (int s = 0; s < kStages; ++s) {
+            for (int s = 0; s < Z::kStages; ++s) {
                 mbar_init(&sh->full[s], 1);
                 mbar_init(&sh->empty[s], 1);
+                mbar_init(&sh->part[s], 1);
+                mbar_init(&sh->ready[s], 1);
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh->acc_full[i], 1);
-                mbar_init(&sh->acc_empty[i], 4);
+                mbar_init(&sh->acc_empty[i], 8);  // four warps of each CTA
             }
             mbar_init(&sh->drain, 1);
             sh->gave_up = 0;
@@ -258,121 +342,167 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
         tma_prefetch_map(&A.b32);
     }
     __syncthreads();
+    cluster_barrier();  // the peer's barriers exist
     tc_fence_after();
 
+    // The producer's and the MMA's loops are single threads, whose few
+    // instructions a stage are serial time of the pipeline: addresses, barriers
+    // and descriptors are stepped, not computed.
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t it = 0;  // stages filled
-            for (int t = blockIdx.x; t < sh->tiles; t += gridDim.x) {
-                const Tile q = tile_at(A, sh, t);
-                bool ok = true;
-                for (int kb = 0; kb < q.depth; kb += kBK, ++it) {
-                    const int s = it % kStages;
-                    if (it >= kStages)
-                        ok = wait_or_give_up(sh, &sh->empty[s], (it / kStages - 1) & 1);
+            Ring<Z::kStages> ring;
+            const uint32_t full0 = map_to_rank(&sh->full[0], 0);  // the leading CTA's
+            const uint32_t part0 = map_to_rank(&sh->part[0], 1);
+            bool ok = true;
+            for (int t = t0; ok && t < sh->tiles; t += dt) {
+                const Tile q = tile_at<BN>(A, sh, t);
+                // this CTA's lanes and its half of the columns
+                const int m0 = q.m0 + rank * kBM;
+                const int half = (q.cols + 31) / 32 * 16, c0 = q.c0 + rank * half;
+                // boxes of 64 columns (MN-major), of 32 or one of all (K-major)
+                const bool narrow = !A.b_mn && half <= 64;
+                const int boxes = A.b_mn ? (half + 63) / 64 : narrow ? (half + 31) / 32 : 1;
+                const int box = A.b_mn ? kBox : (narrow ? 32 : Z::kHalf) * kBK * 2;
+                const int z = A.by_rows ? q.group : 0;
+                const uint32_t bytes = kABytes + boxes * box;
+                const CUtensorMap* const mb = narrow ? &A.b32 : &A.b;
+                const int end = q.k0 + q.depth;
+                const int cleared = cleared_rows(A, (q.depth - 1) % kBK + 1);
+                for (int k = q.k0; k < end; k += kBK) {
+                    if (ring.lap && !mbar_try_wait(&sh->empty[ring.s], ring.lap - 1 & 1))
+                        ok = wait_local(sh, &sh->empty[ring.s], ring.lap - 1 & 1);
                     if (!ok) break;
-                    uint8_t* const sa = stages + s * kStageBytes;
+                    uint8_t* const sa = stages + ring.s * Z::kStageBytes;
                     uint8_t* const sb = sa + kABytes;
-                    uint64_t* const bar = &sh->full[s];
-                    const int z = A.by_rows ? q.group : 0;
-                    const int k = q.k0 + kb;
-                    // columns to bring: 32 at a time (K-major), 64 (MN-major)
-                    const bool narrow = !A.b_mn && q.cols <= kBN / 2;
-                    const int boxes = A.b_mn ? (q.cols + 63) / 64
-                                             : narrow ? (q.cols + 31) / 32 : 1;
-                    const int box = A.b_mn ? 64 * kBK * 2 : narrow ? 32 * kBK * 2 : kBBytes;
-                    mbar_expect_tx(bar, kABytes + boxes * box);
+                    const bool clear = cleared > 0 && k + kBK > end;
+                    uint32_t bar = full0 + ring.s * 8;
+                    if (rank == 0) {
+                        mbar_expect_tx(&sh->full[ring.s], clear ? bytes : 2 * bytes);
+                    } else if (clear) {
+                        mbar_expect_tx(&sh->part[ring.s], bytes);
+                        bar = part0 + ring.s * 8;
+                    }
                     if (A.a_mn) {
-                        tma_load_3d(sa, &A.a, q.m0, k, z, bar);
-                        tma_load_3d(sa + kABytes / 2, &A.a, q.m0 + 64, k, z, bar);
+                        tma_load_3d_pair(sa, &A.a, m0, k, z, bar);
+                        tma_load_3d_pair(sa + kBox, &A.a, m0 + 64, k, z, bar);
                     } else {
-                        tma_load_3d(sa, &A.a, k, q.m0, z, bar);
+                        tma_load_3d_pair(sa, &A.a, k, m0, z, bar);
                     }
                     if (A.b_mn) {
-                        for (int i = 0; i < boxes; ++i)
-                            tma_load_3d(sb + i * box, &A.b, q.c0 + 64 * i, k, 0, bar);
-                    } else if (narrow) {
-                        for (int i = 0; i < boxes; ++i)
-                            tma_load_3d(sb + i * box, &A.b32, k, q.c0 + 32 * i, 0, bar);
+                        tma_load_3d_pair(sb, mb, c0, k, 0, bar);
+                        if (boxes > 1) tma_load_3d_pair(sb + kBox, mb, c0 + 64, k, 0, bar);
                     } else {
-                        tma_load_3d(sb, &A.b, k, q.c0, 0, bar);
+                        tma_load_3d_pair(sb, mb, k, c0, 0, bar);
+                        if (boxes > 1) tma_load_3d_pair(sb + box, mb, k, c0 + 32, 0, bar);
                     }
+                    ring.next();
                 }
-                if (!ok) break;
             }
-            // the copies of the last stages have landed before the CTA may end
-            for (uint32_t i = it > kStages ? it - kStages : 0; i < it; ++i)
-                mbar_wait(&sh->full[i % kStages], (i / kStages) & 1);
+            // Normally every copy has been consumed by the time the pair's last
+            // accumulator is. After a wait that ran out, copies may be in flight
+            // without a barrier of this CTA to tell: leave them a millisecond.
+            if (*reinterpret_cast<volatile int*>(&sh->gave_up))
+                for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         }
+        __syncwarp();
     } else if (warp == 1) {
-        uint32_t it = 0;
+        Ring<Z::kStages> ring;
+        uint32_t parts = 0;  // bit s: phase of part[s] / ready[s]
         int used = 0;
         bool ok = true;
-        const uint32_t sbase = smem_u32(stages);
-        for (int t = blockIdx.x; ok && t < sh->tiles; t += gridDim.x) {
-            const Tile q = tile_at(A, sh, t);
+        const uint32_t sa0 = smem_u32(stages), sb0 = sa0 + kABytes;
+        const uint64_t da0 = A.a_mn ? smem_desc(sa0, kBox, 1024) : smem_desc(sa0, 16, 1024);
+        const uint64_t db0 = A.b_mn ? smem_desc(sb0, kBox, 1024) : smem_desc(sb0, 16, 1024);
+        // a step of 16: 16 rows of 128 bytes, or 32 bytes along them
+        const uint32_t ja = (A.a_mn ? 2048 : 32) >> 4, jb = (A.b_mn ? 2048 : 32) >> 4;
+        for (int t = t0; ok && t < sh->tiles; t += dt) {
+            const Tile q = tile_at<BN>(A, sh, t);
             if (q.depth <= 0) continue;
-            const int buf = used & 1;
-            if (used >= 2) ok = wait_or_give_up(sh, &sh->acc_empty[buf], (used / 2 - 1) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t d = sh->tmem + buf * kBN;
-            const int n = (q.cols + 15) / 16 * 16;
-            const uint32_t idesc = mma_idesc(A.bf16, A.a_mn, A.b_mn, kBM, n);
-            for (int kb = 0; kb < q.depth; kb += kBK, ++it) {
-                const int s = it % kStages;
-                ok = wait_or_give_up(sh, &sh->full[s], (it / kStages) & 1);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t sa = sbase + s * kStageBytes, sb = sa + kABytes;
-                const int left = min(kBK, q.depth - kb), steps = (left + 15) / 16;
-                if (!A.by_rows && left < steps * 16) {
-                    // rows of the next group: both operands cleared, row by row
-                    // (a row is 128 bytes of each box, whatever the swizzle)
-                    const int boxes = 2 + (q.cols + 63) / 64, rows = steps * 16 - left;
-                    uint8_t* const base = stages + s * kStageBytes;
-                    for (int i = lane; i < boxes * rows * 8; i += 32) {
-                        const int x = i / (rows * 8), r = i / 8 % rows;
-                        *reinterpret_cast<uint4*>(base + x * (64 * kBK * 2) +
-                                                  (left + r) * 128 + i % 8 * 16) =
-                            make_uint4(0, 0, 0, 0);
-                    }
-                    fence_async_smem();
-                    __syncwarp();
+            const int n = (q.cols + 31) / 32 * 32;
+            const int blocks = (q.depth + kBK - 1) / kBK;
+            const int left = q.depth - (blocks - 1) * kBK;  // of the last block
+            const int cleared = cleared_rows(A, left);
+            if (rank != 0) {
+                // the second CTA: only what has to be cleared
+                ring.skip(blocks - 1);
+                if (cleared > 0) {
+                    const int st = ring.s;
+                    ok = wait_local_warp(sh, &sh->part[st], parts >> st & 1, lane);
+                    if (!ok) break;
+                    parts ^= 1u << st;
+                    clear_rows(stages + st * Z::kStageBytes, n, left, cleared, lane);
+                    if (lane == 0) mbar_arrive_cluster(map_to_rank(&sh->ready[st], 0));
                 }
+                ring.next();
+                continue;
+            }
+            const int buf = used & 1;
+            if (used >= 2) ok = wait_local_warp(sh, &sh->acc_empty[buf], (used / 2 - 1) & 1, lane);
+            if (!ok) break;
+            const uint32_t d = sh->tmem + buf * BN;
+            const uint32_t idesc = mma_idesc(A.bf16, A.a_mn, A.b_mn, kPairM, n);
+            const int whole = left == kBK ? blocks : blocks - 1;
+            if (lane == 0) {
+                Ring<Z::kStages> r = ring;
+                for (int i = 0; i < whole; ++i) {
+                    if (!mbar_try_wait(&sh->full[r.s], r.lap & 1))
+                        ok = wait_local(sh, &sh->full[r.s], r.lap & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t da = da0 + r.s * (Z::kStageBytes >> 4);
+                    const uint64_t db = db0 + r.s * (Z::kStageBytes >> 4);
+                    mma_f16_pair(d, da, db, idesc, i > 0);
+                    mma_f16_pair(d, da + ja, db + jb, idesc, true);
+                    mma_f16_pair(d, da + 2 * ja, db + 2 * jb, idesc, true);
+                    mma_f16_pair(d, da + 3 * ja, db + 3 * jb, idesc, true);
+                    mma_commit_pair(&sh->empty[r.s]);
+                    r.next();
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+            if (!ok) break;
+            ring.skip(whole);
+            if (whole < blocks) {  // the last block, of fewer steps
+                const int st = ring.s;
+                ok = wait_local_warp(sh, &sh->full[st], ring.lap & 1, lane);
+                if (!ok) break;
+                if (cleared > 0) {
+                    clear_rows(stages + st * Z::kStageBytes, n, left, cleared, lane);
+                    ok = wait_peer_warp(sh, &sh->ready[st], parts >> st & 1, lane);
+                    if (!ok) break;
+                    parts ^= 1u << st;
+                }
+                tc_fence_after();
                 if (lane == 0) {
-                    for (int j = 0; j < steps; ++j) {
-                        const uint64_t da =
-                            A.a_mn ? smem_desc(sa + j * 2048, kABytes / 2, 1024)
-                                   : smem_desc(sa + j * 32, 16, 1024);
-                        const uint64_t db = A.b_mn
-                                                ? smem_desc(sb + j * 2048, 64 * kBK * 2, 1024)
-                                                : smem_desc(sb + j * 32, 16, 1024);
-                        mma_f16(d, da, db, idesc, kb + j > 0);
-                    }
-                    mma_commit(&sh->empty[s]);
+                    const uint64_t da = da0 + st * (Z::kStageBytes >> 4);
+                    const uint64_t db = db0 + st * (Z::kStageBytes >> 4);
+                    for (int j = 0; j < (left + 15) / 16; ++j)
+                        mma_f16_pair(d, da + j * ja, db + j * jb, idesc, whole + j > 0);
+                    mma_commit_pair(&sh->empty[st]);
                 }
                 __syncwarp();
+                ring.next();
             }
-            if (!ok) break;
-            if (lane == 0) mma_commit(&sh->acc_full[buf]);
+            if (lane == 0) mma_commit_pair(&sh->acc_full[buf]);
             __syncwarp();
             ++used;
         }
-        if (!ok) {
-            if (lane == 0) mma_commit(&sh->drain);
+        if (!ok && rank == 0) {
+            if (lane == 0) mma_commit_pair(&sh->drain);
             __syncwarp();
             mbar_wait(&sh->drain, 0);
         }
+        __syncwarp();
     } else {
-        if (A.bf16) epilogue<__nv_bfloat16>(A, sh, warp & 3, lane);
-        else epilogue<__half>(A, sh, warp & 3, lane);
+        if (A.bf16) epilogue<__nv_bfloat16, BN>(A, sh, rank, warp & 3, lane);
+        else epilogue<__half, BN>(A, sh, rank, warp & 3, lane);
     }
     tc_fence_before();
     __syncthreads();
+    cluster_barrier();  // neither CTA reads or signals the other any more
     if (warp == 1) {
         tc_fence_after();
-        tmem_free(sh->tmem, kTmemCols);
+        tmem_free_pair(sh->tmem, Z::kTmemCols);
     }
 }
 
@@ -456,9 +586,15 @@ int encode(CUtensorMap* map, const Operand& o, bool bf16, uint32_t box_rows) {
     return SK_OK;
 }
 
-constexpr size_t kGroupedSmem = 1024 + kStages * kStageBytes + sizeof(GroupedShared);
-static_assert(kGroupedSmem <= 232448, "shared memory of one CTA");
+template <int BN>
+constexpr size_t grouped_smem() {
+    return 1024 + Shape<BN>::kStages * Shape<BN>::kStageBytes + sizeof(GroupedShared);
+}
+static_assert(grouped_smem<256>() <= 232448 && grouped_smem<64>() <= 232448,
+              "shared memory of one CTA");
+static_assert(Shape<256>::kStages <= kMaxStages && Shape<64>::kStages <= kMaxStages, "barriers");
 
+template <int BN>
 int launch_grouped(GroupedArgs& A, Operand a, Operand b, int64_t tiles, char* ws,
                    cudaStream_t s) {
     // the runtime calls first: they bind the device's context to a thread that has
@@ -467,16 +603,27 @@ int launch_grouped(GroupedArgs& A, Operand a, Operand b, int64_t tiles, char* ws
     SK_CUDA(cudaGetDevice(&dev));
     SK_CUDA(cudaSetDevice(dev));
     SK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    SK_CUDA(cudaFuncSetAttribute(k_grouped, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)kGroupedSmem));
+    SK_CUDA(cudaFuncSetAttribute(k_grouped<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)grouped_smem<BN>()));
     int rc = a.pack(ws, s);
     if (rc == SK_OK) rc = b.pack(ws, s);
     if (rc == SK_OK) rc = encode(&A.a, a, A.bf16, A.a_mn ? kBK : kBM);
-    if (rc == SK_OK) rc = encode(&A.b, b, A.bf16, A.b_mn ? kBK : kBN);
+    if (rc == SK_OK) rc = encode(&A.b, b, A.bf16, A.b_mn ? kBK : Shape<BN>::kHalf);
     if (rc == SK_OK) rc = encode(&A.b32, b, A.bf16, A.b_mn ? kBK : 32);
     if (rc != SK_OK) return rc;
-    k_grouped<<<(unsigned)std::min<int64_t>(tiles, sms), kThreads, kGroupedSmem, s>>>(A);
-    SK_LAUNCHED("k_grouped");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, sms / 2));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = grouped_smem<BN>();
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SK_CUDA(cudaLaunchKernelEx(&cfg, k_grouped<BN>, A));
     return SK_OK;
 }
 
@@ -493,8 +640,8 @@ int check_grouped(int dtype, int64_t S, int64_t K, int64_t N, int64_t E, const i
 }
 
 // Tiles of a launch, at most (the runs are known to the device alone).
-int64_t most_tiles(int64_t m, int64_t c, int64_t groups) {
-    return (m + kBM - 1) / kBM * ((c + kBN - 1) / kBN + groups);
+int64_t most_tiles(int64_t m, int64_t c, int64_t groups, int bn) {
+    return (m + kPairM - 1) / kPairM * ((c + bn - 1) / bn + groups);
 }
 
 // W_e's axes as an operand: rows of the unit-stride axis.
@@ -554,11 +701,15 @@ int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ld
     A.a_mn = swn == 1;
     A.b_mn = false;
     A.bf16 = dtype == SK_BF16;
-    const int64_t tiles = most_tiles(N, S, E + 2);
+    const int64_t tiles = most_tiles(N, S, E + 2, 64);
     if (tiles > INT32_MAX) return fail(SK_ERR_ARG, "the output has too many tiles");
-    return launch_grouped(A, weight_operand(w, E, K, N, swe, swk, swn),
-                          Operand{x, 1, S, K, 0, ldx}, tiles, (char*)workspace,
-                          (cudaStream_t)stream);
+    const Operand ow = weight_operand(w, E, K, N, swe, swk, swn);
+    const Operand ox{x, 1, S, K, 0, ldx};
+    // short groups (32 rows on average): narrow tiles, more weights in flight
+    return S <= 32 * E ? launch_grouped<64>(A, ow, ox, tiles, (char*)workspace,
+                                            (cudaStream_t)stream)
+                       : launch_grouped<256>(A, ow, ox, tiles, (char*)workspace,
+                                             (cudaStream_t)stream);
 }
 
 size_t sk_grouped_matmul_weight_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
@@ -595,10 +746,10 @@ int sk_grouped_matmul_weight(const void* x, int dtype, int64_t S, int64_t K, int
     A.m = (int)(transposed ? K : N);
     A.c = (int)(transposed ? N : K);
     A.ldo = A.m;
-    const int64_t tiles = (A.m + kBM - 1) / kBM * (int64_t)((A.c + kBN - 1) / kBN) * E;
+    const int64_t tiles = (A.m + kPairM - 1) / kPairM * (int64_t)((A.c + 255) / 256) * E;
     if (tiles > INT32_MAX) return fail(SK_ERR_ARG, "the output has too many tiles");
-    return launch_grouped(A, transposed ? ox : og, transposed ? og : ox, tiles,
-                          (char*)workspace, (cudaStream_t)stream);
+    return launch_grouped<256>(A, transposed ? ox : og, transposed ? og : ox, tiles,
+                               (char*)workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

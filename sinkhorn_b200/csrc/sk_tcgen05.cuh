@@ -26,34 +26,50 @@ __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, bool a_mn, bool b_mn
            (b_mn ? 1u : 0u) << 16 | (uint32_t)(N >> 3) << 17 | (uint32_t)(M >> 4) << 24;
 }
 
-__device__ __forceinline__ void tmem_alloc(uint32_t* out, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+// cta_group::2: the two CTAs of a cluster of two work on one tile. Allocation
+// and release are joint (a warp of each CTA calls them); the CTA of even rank
+// issues the MMAs, which read both CTAs' shared memory at the same offsets and
+// write both CTAs' tensor memory (each holds its 128 of the 256 lanes).
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* out, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(out)),
                  "r"(columns)
                  : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr),
+__device__ __forceinline__ void tmem_free_pair(uint32_t addr, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr),
                  "r"(columns)
                  : "memory");
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                        bool accumulate) {
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                             bool accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
         : "memory");
 }
 
-// Arrive at `bar` once the MMAs this thread has issued so far are done.
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+// tma_load_3d of a CTA of a pair into its own shared memory, completing on a
+// barrier of either CTA of the pair (a shared::cluster address).
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, int x, int y,
+                                                 int z, uint32_t bar) {
     asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-            smem_u32(bar))
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+// Arrive at `bar` of both CTAs once the MMAs this thread has issued are done.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster"
+        ".b64 [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
         : "memory");
 }
 
