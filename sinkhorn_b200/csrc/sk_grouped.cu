@@ -65,7 +65,7 @@ struct GroupedArgs {
     bool by_rows, a_mn, b_mn, bf16;
 };
 
-struct alignas(8) GroupedShared {
+struct alignas(16) GroupedShared {
     // full (the leading CTA's): the copies of both CTAs of a stage have landed.
     // empty, acc_full: committed by the MMAs to both. A stage whose last rows are
     // cleared takes another way: the second CTA's copies complete on its own
@@ -79,6 +79,7 @@ struct alignas(8) GroupedShared {
     // behind the last; rows in no group are zero
     int first[kMaxGroups + 3];  // first row of each
     int tile0[kMaxGroups + 3];  // first tile of each (by_rows)
+    alignas(16) uint8_t turn[4][2048];  // the epilogue warps' 32 x 32 elements
 };
 
 struct Tile {
@@ -93,14 +94,26 @@ __device__ __forceinline__ bool flagged(GroupedShared* sh, bool ok) {
     if (!ok) *reinterpret_cast<volatile int*>(&sh->gave_up) = 1;
     return ok;
 }
-__device__ __forceinline__ bool wait_local(GroupedShared* sh, uint64_t* bar, uint32_t parity) {
-    return flagged(sh, wait_full(bar, parity, &sh->gave_up));
+// The whole warp waits and agrees on the outcome.
+__device__ __forceinline__ bool wait_warp(GroupedShared* sh, uint64_t* bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, flagged(sh, wait_full(bar, parity, &sh->gave_up)));
 }
-// One lane polls for the warp: 32 would take the barrier unit's time from the
-// copies and commits that complete there.
-__device__ __forceinline__ bool wait_local_warp(GroupedShared* sh, uint64_t* bar, uint32_t parity,
-                                                int lane) {
-    const bool ok = lane != 0 || wait_local(sh, bar, parity);
+// An epilogue warp's wait lasts a tile: one lane looks every half microsecond
+// (polling without a pause costs 2% of the products).
+__device__ __forceinline__ bool wait_idle_warp(GroupedShared* sh, uint64_t* bar, uint32_t parity,
+                                               int lane) {
+    bool ok = true;
+    if (lane == 0) {
+        uint32_t i = 0;
+        while (!mbar_try_wait(bar, parity)) {
+            if (*reinterpret_cast<volatile int*>(&sh->gave_up) || ++i > kWaitPolls) {
+                ok = flagged(sh, false);
+                break;
+            }
+            __nanosleep(500);
+        }
+    }
     return __shfl_sync(0xffffffffu, (int)ok, 0);
 }
 __device__ __forceinline__ bool wait_peer_warp(GroupedShared* sh, uint64_t* bar, uint32_t parity,
@@ -114,18 +127,21 @@ __device__ __forceinline__ int column_tiles(int rows) {
     return (rows + BN - 1) / BN;
 }
 
+// A role's place among the groups: its tiles only go up.
+struct Walk {
+    int group = 0;
+};
+
 // Tile t of the launch.
 template <int BN>
-__device__ __forceinline__ Tile tile_at(const GroupedArgs& A, const GroupedShared* sh, int t) {
+__device__ __forceinline__ Tile tile_at(const GroupedArgs& A, const GroupedShared* sh, int t,
+                                        Walk& walk) {
     Tile q;
     const int nm = (A.m + kPairM - 1) / kPairM;
     if (A.by_rows) {
-        int lo = 0, hi = A.E + 1;  // the last group whose first tile is <= t
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (sh->tile0[mid] <= t) lo = mid;
-            else hi = mid - 1;
-        }
+        int lo = walk.group;  // the last group whose first tile is <= t
+        while (lo <= A.E && sh->tile0[lo + 1] <= t) ++lo;
+        walk.group = lo;
         const int r0 = sh->first[lo], rows = sh->first[lo + 1] - r0;
         const int nc = column_tiles<BN>(rows);
         // even tiles, in bands that reuse what of the weights they have loaded
@@ -206,64 +222,109 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
     if (lane == 0) sh->tiles = A.by_rows ? tiles : A.E * nm * column_tiles<BN>(A.c);
 }
 
+// The accumulators to memory. D has the output's contiguous dimension on the
+// lanes, so 32 x 32 pieces are turned in the warp's corner of shared memory: 16-bit
+// fragments are stored transposed, and leave as 16-byte pieces of output rows, 8
+// rows of 64 bytes to an instruction. Outputs whose rows do not start on 16
+// bytes leave element by element.
 template <typename T, int BN>
 __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh, int rank,
                                          int quarter, int lane) {
     int used = 0;  // accumulators so far
     const uint32_t release0 = map_to_rank(&sh->acc_empty[0], 0);
     const uint32_t release1 = map_to_rank(&sh->acc_empty[1], 0);
+    // 32 rows (columns of D) of 64 bytes, the four 16-byte pieces of a row turned
+    // by the row's bits 1 and 2, which spreads both accesses over all banks
+    uint8_t* const turn = sh->turn[quarter];
+    const uint32_t turn0 = smem_u32(turn);
+    const bool wide = A.ldo % 8 == 0 && A.m % 8 == 0 && A.out_group % 8 == 0 &&
+                      (reinterpret_cast<uintptr_t>(A.out) & 15) == 0;
+    Walk walk;
     for (int t = blockIdx.x / 2; t < sh->tiles; t += gridDim.x / 2) {
-        const Tile q = tile_at<BN>(A, sh, t);
+        const Tile q = tile_at<BN>(A, sh, t, walk);
+        const int m0 = q.m0 + rank * kBM + quarter * 32;  // the warp's lanes
         T* const out = reinterpret_cast<T*>(A.out) +
-                       (A.by_rows ? 0 : q.group * A.out_group) + (int64_t)q.c0 * A.ldo;
-        const int m = q.m0 + rank * kBM + quarter * 32 + lane;
+                       (A.by_rows ? 0 : q.group * A.out_group) + (int64_t)q.c0 * A.ldo + m0;
         const int buf = used & 1;
         bool ok = true;
         if (q.depth > 0) {
-            ok = wait_local_warp(sh, &sh->acc_full[buf], (used >> 1) & 1, lane);
+            ok = wait_idle_warp(sh, &sh->acc_full[buf], (used >> 1) & 1, lane);
             tc_fence_after();
         }
-        // pairs of lanes exchange so that each stores two neighbours of a column
-        const bool paired = A.ldo % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3) == 0;
-        for (int c = 0; c < q.cols; c += 32) {
-            uint32_t v[32];
-            if (q.depth > 0 && ok) {
-                tmem_ld32(sh->tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + c, v);
-                tmem_ld_wait();
-            } else {
-                const float fill = ok ? 0.f : NAN;
+        const bool held = q.depth > 0 && ok;
+        const uint32_t acc = sh->tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN;
+        const uint32_t fill = __float_as_uint(ok ? 0.f : NAN);
+        if (wide) {
+            // piece p = lane % 4 of rows lane / 4 + 8 i
+            const int piece = lane & 3, r0 = lane >> 2;
+            const bool in = m0 + piece * 8 < A.m;
+            T* o = out + (int64_t)r0 * A.ldo + piece * 8;
+            for (int c = 0; c < q.cols; c += 32) {
+                uint32_t v[2][16];
+                if (held) {
+                    tmem_ld16x32(acc + c, v[0]);
+                    tmem_ld16x32(acc + (16u << 16) + c, v[1]);
+                    tmem_ld_wait();
+                } else {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(fill);
-            }
-            if (paired) {
-                const int odd = lane & 1;
-                T* o = out + (int64_t)(c + odd) * A.ldo + (m - odd);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float mine = __uint_as_float(odd ? v[i + 1] : v[i]);
-                    const float send = __uint_as_float(odd ? v[i] : v[i + 1]);
-                    const float other = __shfl_xor_sync(0xffffffffu, send, 1);
-                    const uint32_t w = odd ? pack_pair<T>(other, mine) : pack_pair<T>(mine, other);
-                    if (c + i + odd < q.cols) {
-                        if (m - odd + 1 < A.m) *reinterpret_cast<uint32_t*>(o) = w;
-                        else if (m - odd < A.m)
-                            *reinterpret_cast<uint16_t*>(o) = (uint16_t)w;
-                    }
-                    o += 2 * A.ldo;
+                    for (int i = 0; i < 16; ++i) v[0][i] = v[1][i] = fill;
                 }
-            } else {
+                if (c + 32 >= q.cols && q.depth > 0) {
+                    // the accumulator is read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_signal_cluster(buf ? release1 : release0);
+                }
+                __syncwarp();  // the last piece's reads of `turn` are done
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // lanes 16 h ..
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {  // columns 16 g ..: two fragments
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = pack_pair<T>(__uint_as_float(v[h][8 * g + 2 * i]),
+                                                __uint_as_float(v[h][8 * g + 2 * i + 1]));
+                        // matrix l / 8: its lanes 16 h + 8 (l / 8 % 2), columns 16 g + 8 (l / 16)
+                        const int row = 16 * g + 8 * (lane >> 4) + (lane & 7);
+                        const int p = 2 * h + (lane >> 3 & 1);
+                        st_matrix4_trans(turn0 + row * 64 + ((p ^ (row >> 1 & 3)) << 4), w[0],
+                                         w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = r0 + 8 * i;
+                    const uint4 x = *reinterpret_cast<const uint4*>(
+                        turn + row * 64 + ((piece ^ (row >> 1 & 3)) << 4));
+                    if (in && c + row < q.cols)
+                        *reinterpret_cast<uint4*>(o + (int64_t)i * 8 * A.ldo) = x;
+                }
+                o += 32 * A.ldo;
+            }
+        } else {
+            for (int c = 0; c < q.cols; c += 32) {
+                uint32_t v[32];
+                if (held) {
+                    tmem_ld32(acc + c, v);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = fill;
+                }
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                    if (c + i < q.cols && m < A.m)
-                        out[(int64_t)(c + i) * A.ldo + m] = (T)__uint_as_float(v[i]);
+                    if (c + i < q.cols && m0 + lane < A.m)
+                        out[(int64_t)(c + i) * A.ldo + lane] = (T)__uint_as_float(v[i]);
+            }
+            if (q.depth > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_signal_cluster(buf ? release1 : release0);
             }
         }
-        if (q.depth > 0) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_signal_cluster(buf ? release1 : release0);
-            ++used;
-        }
+        if (q.depth > 0) ++used;
     }
 }
 
@@ -345,33 +406,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
     cluster_barrier();  // the peer's barriers exist
     tc_fence_after();
 
-    // The producer's and the MMA's loops are single threads, whose few
-    // instructions a stage are serial time of the pipeline: addresses, barriers
-    // and descriptors are stepped, not computed.
+    // The producer's and the MMA's few instructions a stage are serial time of the
+    // pipeline (a stage lasts 512 cycles). Both loops are run by whole warps with
+    // one elected lane acting, so that addresses and descriptors stay in uniform
+    // registers; they are stepped, and the next barrier is looked at before the
+    // current stage is issued.
     if (warp == 0) {
-        if (lane == 0) {
-            Ring<Z::kStages> ring;
-            const uint32_t full0 = map_to_rank(&sh->full[0], 0);  // the leading CTA's
-            const uint32_t part0 = map_to_rank(&sh->part[0], 1);
-            bool ok = true;
-            for (int t = t0; ok && t < sh->tiles; t += dt) {
-                const Tile q = tile_at<BN>(A, sh, t);
-                // this CTA's lanes and its half of the columns
-                const int m0 = q.m0 + rank * kBM;
-                const int half = (q.cols + 31) / 32 * 16, c0 = q.c0 + rank * half;
-                // boxes of 64 columns (MN-major), of 32 or one of all (K-major)
-                const bool narrow = !A.b_mn && half <= 64;
-                const int boxes = A.b_mn ? (half + 63) / 64 : narrow ? (half + 31) / 32 : 1;
-                const int box = A.b_mn ? kBox : (narrow ? 32 : Z::kHalf) * kBK * 2;
-                const int z = A.by_rows ? q.group : 0;
-                const uint32_t bytes = kABytes + boxes * box;
-                const CUtensorMap* const mb = narrow ? &A.b32 : &A.b;
-                const int end = q.k0 + q.depth;
-                const int cleared = cleared_rows(A, (q.depth - 1) % kBK + 1);
-                for (int k = q.k0; k < end; k += kBK) {
-                    if (ring.lap && !mbar_try_wait(&sh->empty[ring.s], ring.lap - 1 & 1))
-                        ok = wait_local(sh, &sh->empty[ring.s], ring.lap - 1 & 1);
-                    if (!ok) break;
+        Ring<Z::kStages> ring;
+        const uint32_t full0 = map_to_rank(&sh->full[0], 0);  // the leading CTA's
+        const uint32_t part0 = map_to_rank(&sh->part[0], 1);
+        const bool leader = elect_one();
+        bool ok = true;
+        Walk walk;
+        for (int t = t0; ok && t < sh->tiles; t += dt) {
+            const Tile q = tile_at<BN>(A, sh, t, walk);
+            // this CTA's lanes and its half of the columns
+            const int m0 = q.m0 + rank * kBM;
+            const int half = (q.cols + 31) / 32 * 16, c0 = q.c0 + rank * half;
+            // boxes of 64 columns (MN-major), of 32 or one of all (K-major)
+            const bool narrow = !A.b_mn && half <= 64;
+            const int boxes = A.b_mn ? (half + 63) / 64 : narrow ? (half + 31) / 32 : 1;
+            const int box = A.b_mn ? kBox : (narrow ? 32 : Z::kHalf) * kBK * 2;
+            const int z = A.by_rows ? q.group : 0;
+            const uint32_t bytes = kABytes + boxes * box;
+            const CUtensorMap* const mb = narrow ? &A.b32 : &A.b;
+            const int end = q.k0 + q.depth;
+            const int cleared = cleared_rows(A, (q.depth - 1) % kBK + 1);
+            for (int k = q.k0; k < end; k += kBK) {
+                if (ring.lap) ok = wait_warp(sh, &sh->empty[ring.s], (ring.lap - 1) & 1);
+                if (!ok) break;
+                if (leader) {
                     uint8_t* const sa = stages + ring.s * Z::kStageBytes;
                     uint8_t* const sb = sa + kABytes;
                     const bool clear = cleared > 0 && k + kBK > end;
@@ -395,28 +459,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                         tma_load_3d_pair(sb, mb, k, c0, 0, bar);
                         if (boxes > 1) tma_load_3d_pair(sb + box, mb, k, c0 + 32, 0, bar);
                     }
-                    ring.next();
                 }
+                __syncwarp();
+                ring.next();
             }
-            // Normally every copy has been consumed by the time the pair's last
-            // accumulator is. After a wait that ran out, copies may be in flight
-            // without a barrier of this CTA to tell: leave them a millisecond.
-            if (*reinterpret_cast<volatile int*>(&sh->gave_up))
-                for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         }
+        // Normally every copy has been consumed by the time the pair's last
+        // accumulator is. After a wait that ran out, copies may be in flight
+        // without a barrier of this CTA to tell: leave them a millisecond.
+        if (*reinterpret_cast<volatile int*>(&sh->gave_up))
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         __syncwarp();
     } else if (warp == 1) {
         Ring<Z::kStages> ring;
         uint32_t parts = 0;  // bit s: phase of part[s] / ready[s]
         int used = 0;
         bool ok = true;
+        const bool leader = elect_one();
+        const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem, 0);
         const uint32_t sa0 = smem_u32(stages), sb0 = sa0 + kABytes;
         const uint64_t da0 = A.a_mn ? smem_desc(sa0, kBox, 1024) : smem_desc(sa0, 16, 1024);
         const uint64_t db0 = A.b_mn ? smem_desc(sb0, kBox, 1024) : smem_desc(sb0, 16, 1024);
         // a step of 16: 16 rows of 128 bytes, or 32 bytes along them
         const uint32_t ja = (A.a_mn ? 2048 : 32) >> 4, jb = (A.b_mn ? 2048 : 32) >> 4;
+        Walk walk;
         for (int t = t0; ok && t < sh->tiles; t += dt) {
-            const Tile q = tile_at<BN>(A, sh, t);
+            const Tile q = tile_at<BN>(A, sh, t, walk);
             if (q.depth <= 0) continue;
             const int n = (q.cols + 31) / 32 * 32;
             const int blocks = (q.depth + kBK - 1) / kBK;
@@ -427,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                 ring.skip(blocks - 1);
                 if (cleared > 0) {
                     const int st = ring.s;
-                    ok = wait_local_warp(sh, &sh->part[st], parts >> st & 1, lane);
+                    ok = wait_warp(sh, &sh->part[st], parts >> st & 1);
                     if (!ok) break;
                     parts ^= 1u << st;
                     clear_rows(stages + st * Z::kStageBytes, n, left, cleared, lane);
@@ -437,34 +505,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                 continue;
             }
             const int buf = used & 1;
-            if (used >= 2) ok = wait_local_warp(sh, &sh->acc_empty[buf], (used / 2 - 1) & 1, lane);
+            if (used >= 2) ok = wait_warp(sh, &sh->acc_empty[buf], (used / 2 - 1) & 1);
             if (!ok) break;
-            const uint32_t d = sh->tmem + buf * BN;
+            const uint32_t d = tmem + buf * BN;
             const uint32_t idesc = mma_idesc(A.bf16, A.a_mn, A.b_mn, kPairM, n);
             const int whole = left == kBK ? blocks : blocks - 1;
-            if (lane == 0) {
-                Ring<Z::kStages> r = ring;
-                for (int i = 0; i < whole; ++i) {
-                    if (!mbar_try_wait(&sh->full[r.s], r.lap & 1))
-                        ok = wait_local(sh, &sh->full[r.s], r.lap & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t da = da0 + r.s * (Z::kStageBytes >> 4);
-                    const uint64_t db = db0 + r.s * (Z::kStageBytes >> 4);
+            bool seen = whole > 0 && mbar_try_wait(&sh->full[ring.s], ring.lap & 1);
+            for (int i = 0; i < whole; ++i) {
+                if (!__all_sync(0xffffffffu, seen))
+                    ok = wait_warp(sh, &sh->full[ring.s], ring.lap & 1);
+                if (!ok) break;
+                const int st = ring.s;
+                ring.next();
+                seen = i + 1 < whole && mbar_try_wait(&sh->full[ring.s], ring.lap & 1);
+                tc_fence_after();
+                if (leader) {
+                    const uint64_t da = da0 + st * (Z::kStageBytes >> 4);
+                    const uint64_t db = db0 + st * (Z::kStageBytes >> 4);
                     mma_f16_pair(d, da, db, idesc, i > 0);
                     mma_f16_pair(d, da + ja, db + jb, idesc, true);
                     mma_f16_pair(d, da + 2 * ja, db + 2 * jb, idesc, true);
                     mma_f16_pair(d, da + 3 * ja, db + 3 * jb, idesc, true);
-                    mma_commit_pair(&sh->empty[r.s]);
-                    r.next();
+                    mma_commit_pair(&sh->empty[st]);
                 }
+                __syncwarp();
             }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
             if (!ok) break;
-            ring.skip(whole);
             if (whole < blocks) {  // the last block, of fewer steps
                 const int st = ring.s;
-                ok = wait_local_warp(sh, &sh->full[st], ring.lap & 1, lane);
+                ok = wait_warp(sh, &sh->full[st], ring.lap & 1);
                 if (!ok) break;
                 if (cleared > 0) {
                     clear_rows(stages + st * Z::kStageBytes, n, left, cleared, lane);
@@ -473,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                     parts ^= 1u << st;
                 }
                 tc_fence_after();
-                if (lane == 0) {
+                if (leader) {
                     const uint64_t da = da0 + st * (Z::kStageBytes >> 4);
                     const uint64_t db = db0 + st * (Z::kStageBytes >> 4);
                     for (int j = 0; j < (left + 15) / 16; ++j)
@@ -483,12 +552,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                 __syncwarp();
                 ring.next();
             }
-            if (lane == 0) mma_commit_pair(&sh->acc_full[buf]);
+            if (leader) mma_commit_pair(&sh->acc_full[buf]);
             __syncwarp();
             ++used;
         }
         if (!ok && rank == 0) {
-            if (lane == 0) mma_commit_pair(&sh->drain);
+            if (leader) mma_commit_pair(&sh->drain);
             __syncwarp();
             mbar_wait(&sh->drain, 0);
         }

@@ -73,6 +73,14 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
         : "memory");
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(on));
+    return on != 0;
+}
+
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }
@@ -94,6 +102,27 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
           "=r"(v[31])
         : "r"(addr));
+}
+// 16 lanes x 32 columns as four 16 x 8 fragments: of fragment i, thread t gets in
+// v[4i], v[4i+1] row t / 4, columns 2 (t % 4) and the next, in v[4i+2], v[4i+3]
+// the same columns of row t / 4 + 8.
+__device__ __forceinline__ void tmem_ld16x32(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+          "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+}
+// Four 8 x 8 matrices of 16-bit elements (fragments as above, two columns to a
+// register) to shared memory, transposed: lane l gives the address of row l % 8
+// -- the matrix's column -- of matrix l / 8, 16 bytes each.
+__device__ __forceinline__ void st_matrix4_trans(uint32_t addr, uint32_t a, uint32_t b,
+                                                 uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr),
+                 "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
