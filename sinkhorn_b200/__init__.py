@@ -13,10 +13,11 @@ from .cuda.plan import marginal_error as compute_marginal_error
 from .experts import (ExpertDispatch, combine_rows, dispatch_rows, expert_dispatch,
                       grouped_matmul)
 from .logprobs import RowLogprobs, row_logprobs, token_logprobs
+from .routing import Route, sinkhorn_experts, sinkhorn_route
 from .sinkhorn import SinkhornOutput, sinkhorn
 
 __all__ = ["sinkhorn", "SinkhornOutput", "sinkhorn_differentiable", "SinkhornFunction",
            "compute_marginal_error", "RowLogprobs", "row_logprobs", "token_logprobs",
            "ExpertDispatch", "expert_dispatch", "dispatch_rows", "combine_rows",
-           "grouped_matmul",
+           "grouped_matmul", "Route", "sinkhorn_route", "sinkhorn_experts",
            "__version__"]

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -14,8 +15,28 @@ def ptr(t: Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# the handle of a device's current stream without building a Stream object
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """The device as the current one; nothing to do where it is already."""
+    if device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def needs_grad(*xs) -> bool:
+    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs)
 
 
 def tau_arg(tau: float | None) -> float:
@@ -97,7 +118,18 @@ def indices(x: Tensor, shape: tuple, device, name: str) -> Tensor:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"{name} is on {x.device}, expected {device}")
-    return x.detach().to(torch.int64).contiguous()
+    if x.dtype == torch.int64 and x.is_contiguous():
+        return x
+    return x.to(torch.int64).contiguous()
+
+
+def floats(x: Tensor | None) -> Tensor | None:
+    """A dense float32 tensor outside the autograd graph (None passes through)."""
+    if x is None:
+        return None
+    x = x.detach()
+    return x if x.dtype == torch.float32 and x.is_contiguous() \
+        else x.to(torch.float32).contiguous()
 
 
 def workspace(nbytes: int, device) -> Tensor:

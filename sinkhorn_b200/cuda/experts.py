@@ -20,7 +20,7 @@ def sort_slots(index: Tensor, n_experts: int) -> tuple[Tensor, Tensor, Tensor]:
         return order, position, torch.zeros(n_experts + 1, device=dev, dtype=torch.int32)
     offsets = torch.empty(n_experts + 1, device=dev, dtype=torch.int32)
     lib = T.lib()
-    with torch.cuda.device(dev):
+    with T.on(dev):
         ws = T.workspace(lib.sk_expert_dispatch_workspace_bytes(slots, n_experts), dev)
         rc = lib.sk_expert_dispatch(index.data_ptr(), slots, n_experts, order.data_ptr(),
                                     position.data_ptr(), offsets.data_ptr(), ws.data_ptr(),
@@ -41,7 +41,7 @@ def gather_rows(x: Tensor, position: Tensor, offsets: Tensor) -> Tensor:
     D = x.shape[1]
     rows = torch.empty(t * k, D, device=x.device, dtype=x.dtype)
     if rows.numel():
-        with torch.cuda.device(x.device):
+        with T.on(x.device):
             rc = T.lib().sk_dispatch_rows(
                 x.data_ptr(), T.DTYPES[x.dtype], t, k, D, x.stride(0), position.data_ptr(),
                 offsets.data_ptr(), offsets.numel() - 1, rows.data_ptr(),
@@ -60,7 +60,7 @@ def sum_rows(y: Tensor, position: Tensor, offsets: Tensor, weights: Tensor | Non
         return out
     if not k:
         return out.zero_()
-    with torch.cuda.device(y.device):
+    with T.on(y.device):
         rc = T.lib().sk_combine_rows(
             y.data_ptr(), T.DTYPES[y.dtype], t, k, D, y.stride(0), position.data_ptr(),
             offsets.data_ptr(), offsets.numel() - 1, T.ptr(weights), out.data_ptr(),
@@ -82,7 +82,7 @@ def sum_rows_backward(grad: Tensor, y: Tensor, position: Tensor, offsets: Tensor
         return dy, dw
     if not D:
         return dy, None if dw is None else dw.zero_()
-    with torch.cuda.device(y.device):
+    with T.on(y.device):
         rc = T.lib().sk_combine_rows_backward(
             grad.data_ptr(), y.data_ptr(), T.DTYPES[y.dtype], t, k, D, grad.stride(0),
             y.stride(0), position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
@@ -113,7 +113,7 @@ def product(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
     if not K:
         return y.zero_()
     lib = T.lib()
-    with torch.cuda.device(x.device):
+    with T.on(x.device):
         args = (S, K, x.stride(0), w.data_ptr(), E, N, *_weight_strides(w))
         n = lib.sk_grouped_matmul_workspace_bytes(x.data_ptr(), *args)
         ws = T.workspace(n, x.device) if n else None
@@ -133,7 +133,7 @@ def weight_product(x: Tensor, dy: Tensor, offsets: Tensor, transposed: bool) -> 
         dw.zero_()
     elif dw.numel():
         lib = T.lib()
-        with torch.cuda.device(x.device):
+        with T.on(x.device):
             n = lib.sk_grouped_matmul_weight_workspace_bytes(
                 x.data_ptr(), S, K, x.stride(0), dy.data_ptr(), N, dy.stride(0))
             ws = T.workspace(n, x.device) if n else None

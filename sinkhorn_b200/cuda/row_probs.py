@@ -14,29 +14,31 @@ from .. import _tensors as T
 
 def row_probs(X: Tensor, g: Tensor | None, epsilon: float, negate: bool,
               targets: Tensor | None, top_k: int, mask_a: Tensor | None,
-              mask_b: Tensor | None):
+              mask_b: Tensor | None, lead: tuple, keep: bool):
     """sk_row_logprobs on checked, dense arguments: (lse, logprob, entropy,
-    top_logprob, top_index, stats); logprob / top_* are None when not asked for."""
+    top_logprob, top_index, stats), of shape ``lead`` (B * N rows); logprob / top_*
+    are None when not asked for, stats (for the backward) unless ``keep``."""
     B, N, M = X.shape
     dev = X.device
-
-    def new(*shape, dtype=torch.float32):
-        return torch.empty(shape, device=dev, dtype=dtype)
-
-    lse, entropy, stats = new(B, N), new(B, N), new(B, N, 2)
-    logprob = new(B, N) if targets is not None else None
-    top_lp = new(B, N, top_k) if top_k else None
-    top_idx = new(B, N, top_k, dtype=torch.int64) if top_k else None
+    f32 = torch.float32
+    lse = torch.empty(lead, device=dev, dtype=f32)
+    entropy = torch.empty(lead, device=dev, dtype=f32)
+    stats = torch.empty((B, N, 2), device=dev, dtype=f32) if keep else None
+    logprob = torch.empty(lead, device=dev, dtype=f32) if targets is not None else None
+    top_lp = top_idx = None
+    if top_k:
+        top_lp = torch.empty((*lead, top_k), device=dev, dtype=f32)
+        top_idx = torch.empty((*lead, top_k), device=dev, dtype=torch.int64)
     if B * N:
         lib = T.lib()
-        with torch.cuda.device(dev):
+        with T.on(dev):
             ws = None if mask_b is None else T.workspace(
                 lib.sk_row_logprobs_workspace_bytes(B, M), dev)
             rc = lib.sk_row_logprobs(
                 X.data_ptr(), T.DTYPES[X.dtype], B, N, M, *X.stride(), T.ptr(g), epsilon,
                 int(negate), T.ptr(mask_a), T.ptr(mask_b), T.ptr(targets), top_k,
                 lse.data_ptr(), T.ptr(logprob), entropy.data_ptr(), T.ptr(top_lp),
-                T.ptr(top_idx), stats.data_ptr(), T.ptr(ws), 0 if ws is None else ws.numel(),
+                T.ptr(top_idx), T.ptr(stats), T.ptr(ws), 0 if ws is None else ws.numel(),
                 T.stream_of(dev))
             T.check(rc, "sk_row_logprobs")
     return lse, logprob, entropy, top_lp, top_idx, stats
@@ -54,16 +56,13 @@ def row_probs_backward(X: Tensor, g: Tensor | None, epsilon: float, negate: bool
     dX = torch.empty(B, N, M, device=dev, dtype=X.dtype) if need_dX else None
     dg = torch.empty(B, M, device=dev, dtype=torch.float32) if need_dg else None
 
-    def dense(t):
-        return None if t is None else t.detach().to(torch.float32).contiguous()
-
-    grads = [dense(t) for t in (grad_lse, grad_logprob, grad_entropy, grad_top)]
+    grads = [T.floats(t) for t in (grad_lse, grad_logprob, grad_entropy, grad_top)]
     if not B * N:
         return dX, None if dg is None else dg.zero_()
     if not (need_dX or need_dg):
         return dX, dg
     lib = T.lib()
-    with torch.cuda.device(dev):
+    with T.on(dev):
         ws = T.workspace(lib.sk_row_logprobs_backward_workspace_bytes(B, N, M), dev) \
             if need_dg or mask_b is not None else None
         rc = lib.sk_row_logprobs_backward(

@@ -92,7 +92,7 @@ class DispatchRowsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, position: Tensor, offsets: Tensor) -> Tensor:
         ctx.save_for_backward(position, offsets)
-        return gather_rows(x.detach(), position, offsets)
+        return gather_rows(x, position, offsets)
 
     @staticmethod
     @once_differentiable
@@ -106,19 +106,15 @@ class CombineRowsFunction(torch.autograd.Function):
     def forward(ctx: Any, y: Tensor, weights: Tensor | None, position: Tensor,
                 offsets: Tensor) -> Tensor:
         ctx.save_for_backward(y, weights, position, offsets)
-        return sum_rows(y.detach(), position, offsets, _dense(weights))
+        return sum_rows(y, position, offsets, T.floats(weights))
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: Tensor):
         y, weights, position, offsets = ctx.saved_tensors
-        dy, dw = sum_rows_backward(grad, y.detach(), position, offsets, _dense(weights),
+        dy, dw = sum_rows_backward(grad, y, position, offsets, T.floats(weights),
                                    ctx.needs_input_grad[0], ctx.needs_input_grad[1])
         return dy, None if dw is None else dw.to(weights.dtype), None, None
-
-
-def _dense(weights: Tensor | None) -> Tensor | None:
-    return None if weights is None else weights.detach().to(torch.float32).contiguous()
 
 
 def dispatch_rows(x: Tensor, dispatch: ExpertDispatch) -> Tensor:
@@ -130,6 +126,8 @@ def dispatch_rows(x: Tensor, dispatch: ExpertDispatch) -> Tensor:
     T.check_cuda(x, "x")
     _check_dispatch(dispatch, x.device)
     _check_rows(x, "x", dispatch.position.shape[0])
+    if not T.needs_grad(x):
+        return gather_rows(x, dispatch.position, dispatch.offsets)
     return DispatchRowsFunction.apply(x, dispatch.position, dispatch.offsets)
 
 
@@ -153,6 +151,8 @@ def combine_rows(y: Tensor, dispatch: ExpertDispatch, weights: Tensor | None = N
             raise ValueError(f"weights must have shape {(t, k)}, got {tuple(weights.shape)}")
         if weights.device != y.device:
             raise ValueError(f"weights are on {weights.device}, y is on {y.device}")
+    if not T.needs_grad(y, weights):
+        return sum_rows(y, dispatch.position, dispatch.offsets, T.floats(weights))
     return CombineRowsFunction.apply(y, weights, dispatch.position, dispatch.offsets)
 
 
@@ -160,7 +160,7 @@ class GroupedMatmulFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
         ctx.save_for_backward(x, w, offsets)
-        return product(x.detach(), w.detach(), offsets)
+        return product(x, w, offsets)
 
     @staticmethod
     @once_differentiable
@@ -168,9 +168,9 @@ class GroupedMatmulFunction(torch.autograd.Function):
         x, w, offsets = ctx.saved_tensors
         dx = dw = None
         if ctx.needs_input_grad[0]:
-            dx = product(grad, w.detach().transpose(1, 2), offsets)
+            dx = product(grad, w.transpose(1, 2), offsets)
         if ctx.needs_input_grad[1]:
-            dw = weight_product(x.detach(), grad, offsets, transposed=w.stride(2) != 1)
+            dw = weight_product(x, grad, offsets, transposed=w.stride(2) != 1)
         return dx, dw, None
 
 
@@ -207,5 +207,10 @@ def grouped_matmul(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
         raise ValueError(f"offsets must have shape {(E + 1,)}, got {tuple(offsets.shape)}")
     if offsets.device != x.device:
         raise ValueError(f"offsets are on {offsets.device}, x is on {x.device}")
-    offsets = offsets.detach().to(torch.int32).contiguous()
-    return GroupedMatmulFunction.apply(x, unit_weights(w), offsets)
+    if offsets.dtype == torch.int64:
+        offsets = offsets.clamp(0, x.shape[0]).to(torch.int32)
+    offsets = offsets.contiguous()
+    w = unit_weights(w)
+    if not T.needs_grad(x, w):
+        return product(x, w, offsets)
+    return GroupedMatmulFunction.apply(x, w, offsets)

@@ -51,10 +51,9 @@ class RowLogprobsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, X: Tensor, g: Tensor | None, epsilon: float, negate: bool,
                 targets: Tensor | None, top_k: int, mask_a: Tensor | None,
-                mask_b: Tensor | None):
-        gd = None if g is None else g.detach().to(torch.float32).contiguous()
+                mask_b: Tensor | None, lead: tuple):
         lse, logprob, entropy, top_lp, top_idx, stats = row_probs(
-            X.detach(), gd, epsilon, negate, targets, top_k, mask_a, mask_b)
+            X, T.floats(g), epsilon, negate, targets, top_k, mask_a, mask_b, lead, True)
         ctx.set_materialize_grads(False)
         if top_idx is not None:
             ctx.mark_non_differentiable(top_idx)
@@ -69,25 +68,24 @@ class RowLogprobsFunction(torch.autograd.Function):
         X, g, targets, mask_b, top_idx, stats, entropy = ctx.saved_tensors
         need_X, need_g = ctx.needs_input_grad[:2]
         if all(t is None for t in (g_lse, g_lp, g_ent, g_top)) or not (need_X or need_g):
-            return (None,) * 8
-        gd = None if g is None else g.detach().to(torch.float32).contiguous()
-        dX, dg = row_probs_backward(X.detach(), gd, ctx.epsilon, ctx.negate, targets, mask_b,
+            return (None,) * 9
+        dX, dg = row_probs_backward(X, T.floats(g), ctx.epsilon, ctx.negate, targets, mask_b,
                                     top_idx, stats, entropy, g_lse, g_lp, g_ent, g_top,
                                     need_X, need_g)
-        return (dX, None if dg is None else dg.to(g.dtype)) + (None,) * 6
+        return (dX, None if dg is None else dg.to(g.dtype)) + (None,) * 7
 
 
 def _run(X: Tensor, g: Tensor | None, scale: float, negate: bool, targets: Tensor | None,
-         top_k: int, mask_a: Tensor | None, mask_b: Tensor | None):
+         top_k: int, mask_a: Tensor | None, mask_b: Tensor | None, lead: tuple):
     if X.stride(2) != 1 and X.shape[2] > 1:
         X = X.contiguous()  # the kernels read rows of unit column stride
     elif X.stride(2) != 1:
         X = X.as_strided(X.shape, (X.stride(0), X.stride(1), 1))
-    if torch.is_grad_enabled() and (X.requires_grad or (g is not None and g.requires_grad)):
-        return RowLogprobsFunction.apply(X, g, scale, negate, targets, top_k, mask_a, mask_b)
-    if g is not None:
-        g = g.detach().to(torch.float32).contiguous()
-    return row_probs(X.detach(), g, scale, negate, targets, top_k, mask_a, mask_b)[:5]
+    if T.needs_grad(X, g):
+        return RowLogprobsFunction.apply(X, g, scale, negate, targets, top_k, mask_a, mask_b,
+                                         lead)
+    return row_probs(X, T.floats(g), scale, negate, targets, top_k, mask_a, mask_b, lead,
+                     False)[:5]
 
 
 def _check_top_k(top_k: int, M: int) -> int:
@@ -132,14 +130,20 @@ def row_logprobs(C: Tensor, g: Tensor | None = None, epsilon: float = 0.1,
     top_k = _check_top_k(top_k, M)
     epsilon = _check_scale(epsilon, "epsilon")
     if g is not None:
-        T.vec(g, (B, M), C.device, "g")
+        if not isinstance(g, Tensor):
+            raise TypeError("g must be a torch.Tensor or None")
+        if tuple(g.shape) != (B, M):
+            raise ValueError(f"g must have shape {(B, M)}, got {tuple(g.shape)}")
+        if g.device != C.device:
+            raise ValueError(f"g is on {g.device}, C is on {C.device}")
         if not g.dtype.is_floating_point:
             raise TypeError(f"g must be a floating point tensor, got {g.dtype}")
     if targets is not None:
         targets = T.indices(targets, (B, N), C.device, "targets")
     ma = T.mask(mask_a, (B, N), C.device, "mask_a")
     mb = T.mask(mask_b, (B, M), C.device, "mask_b")
-    lse, logprob, entropy, top_lp, top_idx = _run(C, g, epsilon, True, targets, top_k, ma, mb)
+    lse, logprob, entropy, top_lp, top_idx = _run(C, g, epsilon, True, targets, top_k, ma, mb,
+                                                  (B, N))
     return RowLogprobs(lse, entropy, logprob, top_lp, top_idx)
 
 
@@ -171,13 +175,6 @@ def token_logprobs(logits: Tensor, targets: Tensor | None = None, top_k: int = 0
         X = logits.unsqueeze(0)
     else:
         X = logits.reshape(1, math.prod(lead), V)
-    if targets is not None:
-        targets = targets.reshape(X.shape[:2])
     lse, logprob, entropy, top_lp, top_idx = _run(X, None, temperature, False, targets, top_k,
-                                                  None, None)
-
-    def shape(t, *more):
-        return None if t is None else t.reshape(*lead, *more)
-
-    return RowLogprobs(shape(lse), shape(entropy), shape(logprob), shape(top_lp, top_k),
-                       shape(top_idx, top_k))
+                                                  None, None, lead)
+    return RowLogprobs(lse, entropy, logprob, top_lp, top_idx)

@@ -26,6 +26,7 @@ from . import _tensors as T
 from .autograd import TransportPlanFunction, _check_backend, sinkhorn_differentiable
 from .cuda import plan as _plan
 from .cuda.forward import sinkhorn_forward_cuda
+from .logprobs import RowLogprobs, row_logprobs
 
 
 def _needs_grad(*xs) -> bool:
@@ -62,6 +63,15 @@ class SinkhornOutput:
             P = self.transport_plan(C, epsilon)
             return (P * C).sum(dim=(-2, -1))
         return _plan.cost(C, self.f, self.g, epsilon).to(C.dtype)
+
+    def assign(self, C: Tensor, epsilon: float, top_k: int = 1,
+               targets: Tensor | None = None, mask_a: Tensor | None = None,
+               mask_b: Tensor | None = None) -> RowLogprobs:
+        """Each row's distribution over the columns under the plan (its rows
+        normalised), from C and g alone: the top_k columns with their log
+        probabilities, the entropy, and the log probability of a given column
+        (``row_logprobs``; the plan is not stored)."""
+        return row_logprobs(C, self.g, epsilon, targets, top_k, mask_a, mask_b)
 
     def sinkhorn_divergence(self, C: Tensor, epsilon: float, a: Tensor | None = None,
                             b: Tensor | None = None) -> Tensor:
