@@ -22,6 +22,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cooperative_groups.h>
+#include <float.h>
 #include <limits.h>
 
 #include <algorithm>
@@ -29,6 +30,7 @@
 
 #include "sk_common.cuh"
 #include "sk_internal.h"
+#include "sk_tma.cuh"
 
 namespace sk {
 namespace {
@@ -44,8 +46,13 @@ constexpr float kFarBelow = -1e4f;
 struct RowProbArgs {
     const void* X;
     int64_t N, M, sXb, sXn;
-    int64_t rows;           // B * N
+    int64_t B;
+    int per_cta;            // rows of one item to a CTA
+    unsigned groups;        // CTAs of an item
+    int stages;             // of each warp's ring
+    bool staged;            // each CTA holds g (and mask_b) in shared memory
     const float* g;         // (B,M) or NULL; -inf where mask_b leaves a column out
+    const uint8_t* mask_b;  // (B,M) or NULL: still to be folded in (staged)
     const uint8_t* mask_a;  // (B,N) or NULL
     float sign;             // x = g + sign * X
     float k;                // 1 / eps
@@ -75,16 +82,20 @@ __device__ __forceinline__ uint4 ld_stream16(const void* p) {
 }
 
 // How a value becomes x. kPlain: the element itself. kAffine: g_j + sign * X.
-// kMasked: the same, and -inf where g_j is -inf whatever X holds. A column mask
-// is folded into g once a call (k_masked_g): in the rows' loop a byte mask cost
-// as much as all the rest (16 x 2048 x 2048 fp32 on a B200: 154 us against 93 us
-// with g alone and 53 us with neither).
+// kMasked: the same, and -inf where g_j is -inf whatever X holds: a column mask is
+// folded into g beforehand, because in the rows' loop a byte mask cost as much as
+// all the rest (16 x 2048 x 2048 fp32 on a B200: 154 us against 93 us with g
+// alone). g is read from shared memory where it fits: loads from L1 come back
+// behind the row's own, out of DRAM (115 us against 60 us without g).
 enum Shape { kPlain = 0, kAffine = 1, kMasked = 2 };
+
+extern __shared__ __align__(16) float staged_g[];
 
 struct RowShape {
     const float* g;  // this item's, or NULL
     float sign;
-    bool g16;  // g is 16-byte aligned at the row's vectors
+    bool staged;  // g is in staged_g
+    bool vec;     // g is 16-byte aligned at the row's vectors
 };
 
 template <int SHAPE>
@@ -96,7 +107,8 @@ __device__ __forceinline__ float shaped1(float v, float g, float sign) {
 template <int SHAPE>
 __device__ __forceinline__ float shaped(float v, const RowShape& rs, int64_t j) {
     if (SHAPE == kPlain) return v;
-    return shaped1<SHAPE>(v, rs.g ? __ldg(rs.g + j) : 0.f, rs.sign);
+    const float g = rs.staged ? staged_g[j] : rs.g ? __ldg(rs.g + j) : 0.f;
+    return shaped1<SHAPE>(v, g, rs.sign);
 }
 
 // 2 * V2 consecutive values from column j on.
@@ -104,10 +116,23 @@ template <int SHAPE, int V2>
 __device__ __forceinline__ void shape_pairs(float2* x, const RowShape& rs, int64_t j) {
     if (SHAPE == kPlain) return;
     float2 g[V2];
-    if (!rs.g) {
+    if (rs.staged) {
+        const float* const p = staged_g + j;
+        if (rs.vec) {
+#pragma unroll
+            for (int e = 0; e < V2; e += 2) {
+                const float4 v = *reinterpret_cast<const float4*>(p + 2 * e);
+                g[e] = make_float2(v.x, v.y);
+                g[e + 1] = make_float2(v.z, v.w);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V2; ++e) g[e] = make_float2(p[2 * e], p[2 * e + 1]);
+        }
+    } else if (!rs.g) {
 #pragma unroll
         for (int e = 0; e < V2; ++e) g[e] = make_float2(0.f, 0.f);
-    } else if (rs.g16) {
+    } else if (rs.vec) {
 #pragma unroll
         for (int e = 0; e < V2; e += 2) {
             const float4 v = ld_vec4(rs.g + j + 2 * e);
@@ -131,12 +156,24 @@ __device__ __forceinline__ void shape_pairs(float2* x, const RowShape& rs, int64
 }
 
 __device__ __forceinline__ RowShape row_shape(const float* g, float sign, int64_t b, int64_t M,
-                                              int64_t lead) {
+                                              int64_t lead, bool staged = false) {
     RowShape rs;
     rs.g = g ? g + b * M : nullptr;
     rs.sign = sign;
-    rs.g16 = (reinterpret_cast<uintptr_t>(rs.g + lead) & 15) == 0;
+    rs.staged = staged;
+    rs.vec = staged ? (lead & 3) == 0 : (reinterpret_cast<uintptr_t>(rs.g + lead) & 15) == 0;
     return rs;
+}
+
+__host__ __device__ constexpr int align16(int bytes) { return (bytes + 15) / 16 * 16; }
+
+// An item's g with its mask folded in, into staged_g, by the CTA.
+__device__ __forceinline__ void stage_g(const RowProbArgs& A, int64_t b, int threads) {
+    for (int j = threadIdx.x; j < (int)A.M; j += threads) {
+        const float v = A.g ? A.g[b * A.M + j] : 0.f;
+        staged_g[j] = A.mask_b && !A.mask_b[b * A.M + j] ? kNegInf : v;
+    }
+    __syncthreads();
 }
 
 // g with -inf at the columns that mask_b leaves out.
@@ -201,16 +238,27 @@ struct Moments {
         }
         if (mn != m) move_to(mn, k2);
         const float2 nm = make_float2(-mn, -mn), kk = make_float2(k2, k2);
-        float2 ss = make_float2(0.f, 0.f), uu = ss;
+        constexpr int C = V2 >= 8 ? V2 / 4 : 1;  // chains of sums side by side
+        float2 ss[C], uu[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) ss[c] = uu[c] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < V2; ++e) {
             const float2 y = __fmul2_rn(__fadd2_rn(x[e], nm), kk);
             const float2 t = make_float2(ex2(y.x), ex2(y.y));
-            ss = __fadd2_rn(ss, t);
-            uu = __ffma2_rn(
-                t, BOUND ? make_float2(fmaxf(y.x, kFarBelow), fmaxf(y.y, kFarBelow)) : y, uu);
+            ss[e % C] = __fadd2_rn(ss[e % C], t);
+            uu[e % C] = __ffma2_rn(
+                t, BOUND ? make_float2(fmaxf(y.x, kFarBelow), fmaxf(y.y, kFarBelow)) : y,
+                uu[e % C]);
         }
-        float du = uu.x + uu.y;
+#pragma unroll
+        for (int c = C / 2; c > 0; c /= 2)
+#pragma unroll
+            for (int i = 0; i < c; ++i) {
+                ss[i] = __fadd2_rn(ss[i], ss[i + c]);
+                uu[i] = __fadd2_rn(uu[i], uu[i + c]);
+            }
+        float du = uu[0].x + uu[0].y;
         if (!BOUND && isnan(du)) {
             // 0 * -inf (or a NaN value): once more with the exponents bounded
             du = 0.f;
@@ -221,7 +269,7 @@ struct Moments {
                 du = fmaf(ex2(y.y), fmaxf(y.y, kFarBelow), du);
             }
         }
-        s += ss.x + ss.y;
+        s += ss[0].x + ss[0].y;
         u += du;
     }
 };
@@ -261,36 +309,25 @@ __device__ __forceinline__ bool beats(float v, int i, float w, int j) {
 
 constexpr int kListCap = 128;  // entries of a warp's list, four to a lane
 
-// A warp's candidates for the best k, in shared memory, in any order.
-struct TopList {
-    float* v;
-    int* i;
-    int n = 0;
-    float kth = kNegInf;  // the k-th when the list was last sorted
-    int kth_i = INT_MAX;
-
-    // Sort, keep the best k.
-    __device__ __forceinline__ void keep(int k, int lane) {
-        if (n <= 32) {
-            __syncwarp();
-            const float ev = lane < n ? v[lane] : kNegInf;
-            const int ei = lane < n ? i[lane] : INT_MAX;
-            int rank = lane < n ? 0 : 32;
-            for (int l = 0; l < n; ++l)
-                rank += beats(__shfl_sync(0xffffffffu, ev, l), __shfl_sync(0xffffffffu, ei, l),
-                              ev, ei);
-            if (rank < k) {
-                v[rank] = ev;
-                i[rank] = ei;
-            }
-            __syncwarp();
-            n = min(n, k);
-            return;  // (kth serves a list that ran full)
+// Sort a warp's list of n entries in shared memory and keep the best k; the
+// number kept. (Out of line: it is called where a list is full and once a row.)
+__device__ __noinline__ int keep_best(float* v, int* i, int n, int k, int lane) {
+    __syncwarp();
+    if (n <= 32) {
+        const float ev = lane < n ? v[lane] : kNegInf;
+        const int ei = lane < n ? i[lane] : INT_MAX;
+        int rank = lane < n ? 0 : 32;
+        for (int l = 0; l < n; ++l)
+            rank +=
+                beats(__shfl_sync(0xffffffffu, ev, l), __shfl_sync(0xffffffffu, ei, l), ev, ei);
+        if (rank < k) {
+            v[rank] = ev;
+            i[rank] = ei;
         }
+    } else {
         constexpr int P = kListCap / 32;
         float ev[P];
         int ei[P], rank[P];
-        __syncwarp();
 #pragma unroll
         for (int q = 0; q < P; ++q) {
             const bool in = q * 32 + lane < n;
@@ -302,8 +339,7 @@ struct TopList {
             const float w = v[j];
             const int wi = i[j];
 #pragma unroll
-            for (int q = 0; q < P; ++q)
-                if (q * 32 < n) rank[q] += beats(w, wi, ev[q], ei[q]);
+            for (int q = 0; q < P; ++q) rank[q] += beats(w, wi, ev[q], ei[q]);
         }
         __syncwarp();
 #pragma unroll
@@ -312,13 +348,20 @@ struct TopList {
                 v[rank[q]] = ev[q];
                 i[rank[q]] = ei[q];
             }
-        __syncwarp();
-        n = min(n, k);
-        if (n == k) {
-            kth = v[k - 1];
-            kth_i = i[k - 1];
-        }
     }
+    __syncwarp();
+    return min(n, k);
+}
+
+// A warp's candidates for the best k, in shared memory, in any order.
+struct TopList {
+    float* v;
+    int* i;
+    int n = 0;
+    float kth = kNegInf;  // the k-th when the list last ran full
+    int kth_i = INT_MAX;
+
+    __device__ __forceinline__ void keep(int k, int lane) { n = keep_best(v, i, n, k, lane); }
     // One candidate a lane; -inf, NaN, what is below `floor` and what does not
     // beat the k-th entry are passed over.
     __device__ __forceinline__ void offer(float cv, int ci, int k, float floor, int lane) {
@@ -326,7 +369,9 @@ struct TopList {
         unsigned who = __ballot_sync(0xffffffffu, in);
         if (!who) return;
         if (n + __popc(who) > kListCap) {
-            keep(k, lane);
+            keep(k, lane);  // (more than k were in it)
+            kth = v[k - 1];
+            kth_i = i[k - 1];
             in = in && beats(cv, ci, kth, kth_i);
             who = __ballot_sync(0xffffffffu, in);
         }
@@ -337,9 +382,40 @@ struct TopList {
         }
         n += __popc(who);
     }
+    // Of the lane's 2 * P values those from `floor` on (mostly one or none);
+    // column(e): the column of value e.
+    template <int P, typename F>
+    __device__ __forceinline__ void offer_pairs(const float2* x, F column, int k, float floor,
+                                                int lane) {
+        unsigned marks = 0;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            if (x[e].x >= floor) marks |= 1u << (2 * e);
+            if (x[e].y >= floor) marks |= 2u << (2 * e);
+        }
+        if (kth >= floor) {
+            // the list ran full: rows of equal values end here
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                if (!beats(x[e].x, column(2 * e), kth, kth_i)) marks &= ~(1u << (2 * e));
+                if (!beats(x[e].y, column(2 * e + 1), kth, kth_i)) marks &= ~(2u << (2 * e));
+            }
+        }
+        while (__any_sync(0xffffffffu, marks != 0)) {
+            float w = kNegInf;
+            const int at = marks ? __ffs(marks) - 1 : 0;
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                if (at == 2 * e) w = x[e].x;
+                if (at == 2 * e + 1) w = x[e].y;
+            }
+            offer(marks ? w : kNegInf, column(at), k, floor, lane);
+            marks &= marks - 1;
+        }
+    }
 };
 
-constexpr int kRowWarps = 8;  // warps of a CTA
+constexpr int kRowWarps = 8;  // most warps of a CTA
 
 // 16 bytes of elements as pairs.
 __device__ __forceinline__ void unpack2(const uint4& v, float2* x, const float*) {
@@ -360,32 +436,43 @@ __device__ __forceinline__ void unpack2(const uint4& v, float2* x, const T* t) {
     x[3] = pair_of(v.w, t);
 }
 
-template <bool TOP>
-struct RowProbShared {
-    float m[kRowWarps], s[kRowWarps], u[kRowWarps];
+constexpr int kStash = 32;
+
+// What the W warps of a row share.
+template <bool TOP, int W>
+struct RowShared {
+    float m[W], s[W], u[W];
 };
-template <>
-struct RowProbShared<true> {
-    float m[kRowWarps], s[kRowWarps], u[kRowWarps];
-    float high[kRowWarps * 4];  // the four largest lane maxima of each warp
-    int from[kRowWarps][32];    // first vectors of the lanes that are read again
-    int n[kRowWarps];
-    float lv[kRowWarps][kListCap];
-    int li[kRowWarps][kListCap];
-    float ov[32];  // this CTA's best k, sorted
+template <int W>
+struct RowShared<true, W> {
+    float m[W], s[W], u[W];
+    float high[32];    // the largest lane maxima of each warp, 32 in all
+    int from[W][32];   // first vectors of the lanes that are read again
+    int n[W];
+    float lv[W][kListCap];
+    int li[W][kListCap];
+    float ov[32];  // the best k, sorted
     int oi[32];
 };
 
-// The best k of `lists` unsorted lists of at most 32 entries into ov / oi
-// (-inf and -1 where there are fewer). All threads of the CTA.
-__device__ __forceinline__ void select_best(RowProbShared<true>& sh, int lists, int k) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int total = 0, before = 0;
-    for (int l = 0; l < lists; ++l) {
-        if (l < warp) before += sh.n[l];
-        total += sh.n[l];
-    }
-    if (threadIdx.x < 32) {
+// Vectors with a candidate, of rows that are held in registers.
+template <bool ON>
+struct RowStash {};
+template <>
+struct RowStash<true> {
+    uint4 v[kRowWarps][kStash];
+    int at[kRowWarps][kStash], n[kRowWarps];
+};
+
+// The best k of `lists` unsorted lists of at most 32 entries into ov / oi (-inf
+// and -1 where there are fewer), by the row's warps, at least as many as lists;
+// `sync` is their barrier.
+template <int W, typename Sync>
+__device__ __forceinline__ void select_best(RowShared<true, W>& sh, int lists, int k, int warp,
+                                            int lane, Sync sync) {
+    int total = 0;
+    for (int l = 0; l < lists; ++l) total += sh.n[l];
+    if (warp == 0) {
         sh.ov[lane] = kNegInf;
         sh.oi[lane] = -1;
     }
@@ -412,7 +499,7 @@ __device__ __forceinline__ void select_best(RowProbShared<true>& sh, int lists, 
             }
         }
     } else {
-        __syncthreads();
+        sync();
         if (warp < lists && lane < sh.n[warp]) {
             const float v = sh.lv[warp][lane];
             const int i = sh.li[warp][lane];
@@ -426,229 +513,62 @@ __device__ __forceinline__ void select_best(RowProbShared<true>& sh, int lists, 
             }
         }
     }
-    __syncthreads();
+    sync();
 }
 
-// WARPS == 1: a warp per row, 8 rows per CTA, no cluster. WARPS == 8: a CTA or
-// a cluster of CTAs per row, joined over distributed shared memory by rank 0.
-// A step is U vectors of 16 bytes a lane; as each pair of them is unpacked, the
-// loads of the next step take its registers, so that a warp keeps U KB / 2 in
-// flight. U == 1 is for rows of a single step (and keeps its values).
-template <typename T, int SHAPE, bool TOP, int WARPS, int U>
-__global__ void __launch_bounds__(256, SHAPE ? 3 : 4) k_row_probs(const RowProbArgs A) {
-    constexpr int V = Vec<T>::n;
-    constexpr int H = U == 1 ? 1 : 16 / V;  // vectors folded at once: 16 values
-    static_assert(U % H == 0, "whole folds");
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    __shared__ RowProbShared<TOP> sh;
-    int64_t row;
-    int part = 0, parts = 1;
-    if (WARPS == 1) {
-        row = (int64_t)blockIdx.x * kRowWarps + warp;
-        if (row >= A.rows) return;
-    } else {
-        parts = cg::this_cluster().num_blocks();
-        part = cg::this_cluster().block_rank();
-        row = blockIdx.x / parts;
+// W warps' lane maxima to a value that at least k lanes reach: 32 / W maxima of
+// each warp stand for its lanes.
+template <int W, typename Sync>
+__device__ __forceinline__ float lane_bound(RowShared<true, W>& sh, float best, int k, int warp,
+                                            int lane, Sync sync) {
+    if (W == 1) return fmaxf(warp_rth_largest(best, k, lane), -FLT_MAX);
+    constexpr int HI = 32 / W;
+    unsigned o = ordered(best), mine = 0;
+#pragma unroll
+    for (int q = 0; q < HI; ++q) {
+        const unsigned t = __reduce_max_sync(0xffffffffu, o);
+        if (lane == q) mine = t;
+        if (lane == __ffs(__ballot_sync(0xffffffffu, o == t)) - 1) o = 0;
     }
-    const int64_t b = row / A.N, n = row - b * A.N;
-    const T* const X = reinterpret_cast<const T*>(A.X) + b * A.sXb + n * A.sXn;
-    const int M = (int)A.M;
-    const int lead = (int)row_lead(X, A.M);
-    const RowShape rs = row_shape(A.g, A.sign, b, A.M, lead);
-    const float k2 = A.k * kLog2e;
-    const bool empty = A.mask_a && !A.mask_a[row];
-    const int nv = empty ? 0 : (M - lead) / V;
-    const int k = A.top_k;
-    const int wid = WARPS == 1 ? 0 : part * WARPS + warp;
-    const int step = (WARPS == 1 ? 1 : parts * WARPS) * 32 * U;
+    if (lane < HI) sh.high[warp * HI + lane] = unordered(mine);
+    sync();
+    return fmaxf(warp_rth_largest(sh.high[lane], k, lane), -FLT_MAX);
+}
+
+// Read the vectors of the warp's lanes that reach `bound` again, one to each lane
+// at a time: lane l's are base0 + l + q * 32 + c * step, q < U.
+template <typename T, int SHAPE, int U>
+__device__ __forceinline__ void offer_again(TopList& top, int* from, float best, float bound,
+                                            const T* X, const RowShape& rs, int lead, int nv,
+                                            int base0, int step, int k, int lane) {
+    constexpr int V = Vec<T>::n, V2 = V / 2;
+    const bool held = best >= bound;
+    const unsigned who = __ballot_sync(0xffffffffu, held);
+    if (held) from[__popc(who & ((1u << lane) - 1u))] = base0 + lane;
+    __syncwarp();
+    const int per = (nv - base0 + step - 1) / step * U;  // of a lane, at most
+    const int all = __popc(who) * per;
     const uint4* const body = reinterpret_cast<const uint4*>(X + lead);
-
-    Moments mo;
-    float best = kNegInf;  // the lane's largest value among whole vectors
-    float2 x[H * V / 2];
-
-    auto fold = [&]() {
-        float cm = kNegInf;
-#pragma unroll
-        for (int e = 0; e < H * V / 2; ++e) cm = fmaxf(cm, fmaxf(x[e].x, x[e].y));
-        if (TOP) best = fmaxf(best, cm);
-        mo.fold<SHAPE != kPlain>(x, cm, k2);
-    };
-    const int base = wid * 32 * U + lane;
-    int i = base;  // this lane's first vector of the step
-    if (U > 1 && wid * 32 * U + 32 * U <= nv) {
-        uint4 raw[U];
-#pragma unroll
-        for (int q = 0; q < U; ++q) raw[q] = ld_stream16(body + i + q * 32);
-        const int last = nv - (32 * U - lane);  // of the steps that are whole
-        while (true) {
-            const bool more = i + step <= last;
-#pragma unroll
-            for (int h = 0; h < U; h += H) {
-#pragma unroll
-                for (int q = 0; q < H; ++q) {
-                    unpack2(raw[h + q], x + q * (V / 2), X);
-                    if (more) raw[h + q] = ld_stream16(body + i + step + (h + q) * 32);
-                    shape_pairs<SHAPE, V / 2>(x + q * (V / 2), rs,
-                                             lead + (int64_t)(i + (h + q) * 32) * V);
-                }
-                fold();
-            }
-            i += step;
-            if (!more) break;
-        }
-    }
-    // the warp's last step, vector by vector
-    for (; i - lane < nv; i += step) {
-#pragma unroll
-        for (int h = 0; h < U; h += H) {
-#pragma unroll
-            for (int q = 0; q < H; ++q) {
-                const int at = i + (h + q) * 32;
-                float2* const xq = x + q * (V / 2);
-                if (at < nv) {
-                    unpack2(ld_stream16(body + at), xq, X);
-                    shape_pairs<SHAPE, V / 2>(xq, rs, lead + (int64_t)at * V);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V / 2; ++e) xq[e] = make_float2(kNegInf, kNegInf);
-                }
-            }
-            fold();
-        }
-    }
-    // the row's ends, one column to a lane: up to V - 1 before the first vector
-    // and as many behind the last
-    const int tail = lead + nv * V;
-    float end = kNegInf;
-    int end_j = 0;
-    if (!empty && wid == 0 && (lead > 0 || tail < M)) {
-        end_j = lane < 16 ? lane : tail + lane - 16;
-        if (lane < 16 ? lane < lead : end_j < M) end = shaped<SHAPE>(widen(X[end_j]), rs, end_j);
-        const float2 e[1] = {make_float2(end, kNegInf)};
-        mo.fold<true>(e, end, k2);
-    }
-    mo.join(k2);
-
-    TopList top;
-    if constexpr (TOP) {
-        top.v = sh.lv[warp];
-        top.i = sh.li[warp];
-        top.offer(end, end_j, k, kNegInf, lane);
-        if (U == 1) {
-            const float bound = warp_rth_largest(best, k, lane);
-#pragma unroll
-            for (int e = 0; e < V / 2; ++e) {
-                const bool in = best >= bound && base < nv;
-                top.offer(in ? x[e].x : kNegInf, lead + base * V + 2 * e, k, bound, lane);
-                top.offer(in ? x[e].y : kNegInf, lead + base * V + 2 * e + 1, k, bound, lane);
-            }
+    for (int c = 0; c < all; c += 32) {
+        const int f = c + lane, q = f / per, s = f - q * per;
+        const int at = f < all ? from[q] + s / U * step + s % U * 32 : nv;
+        float2 y[V2];
+        if (at < nv) {
+            unpack2(ld_stream16(body + at), y, X);
+            shape_pairs<SHAPE, V2>(y, rs, lead + (int64_t)at * V);
         } else {
-            float bound;
-            if (WARPS == 1) {
-                bound = warp_rth_largest(best, k, lane);
-            } else {
-                // four maxima of each warp stand for its lanes: k of these 32 are
-                // k lanes, too
-                unsigned o = ordered(best), high = 0;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const unsigned t = __reduce_max_sync(0xffffffffu, o);
-                    if (lane == r) high = t;
-                    if (lane == __ffs(__ballot_sync(0xffffffffu, o == t)) - 1) o = 0;
-                }
-                if (lane < 4) sh.high[warp * 4 + lane] = unordered(high);
-                __syncthreads();
-                bound = warp_rth_largest(sh.high[lane], k, lane);
-            }
-            const bool held = best >= bound && best > kNegInf;
-            const unsigned mine = __ballot_sync(0xffffffffu, held);
-            // the vectors of those lanes, one to each lane of the warp at a time
-            if (held) sh.from[warp][__popc(mine & ((1u << lane) - 1u))] = base;
-            __syncwarp();
-            const int per = (nv - wid * 32 * U + step - 1) / step * U;  // of a lane, at most
-            const int all = __popc(mine) * per;
-            for (int c = 0; c < all; c += 32) {
-                const int f = c + lane, q = f / per, r = f - q * per;
-                const int at = f < all ? sh.from[warp][q] + r / U * step + r % U * 32 : nv;
-                float2 y[V / 2];
-                if (at < nv) {
-                    unpack2(ld_stream16(body + at), y, X);
-                    shape_pairs<SHAPE, V / 2>(y, rs, lead + (int64_t)at * V);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V / 2; ++e) y[e] = make_float2(kNegInf, kNegInf);
-                }
-                unsigned marks = 0;  // values that pass (mostly one or none)
-#pragma unroll
-                for (int e = 0; e < V / 2; ++e) {
-                    if (y[e].x >= bound) marks |= 1u << (2 * e);
-                    if (y[e].y >= bound) marks |= 2u << (2 * e);
-                }
-                while (__any_sync(0xffffffffu, marks != 0)) {
-                    float v = kNegInf;
-                    const int e = marks ? __ffs(marks) - 1 : 0;
-#pragma unroll
-                    for (int p = 0; p < V / 2; ++p) {
-                        if (e == 2 * p) v = y[p].x;
-                        if (e == 2 * p + 1) v = y[p].y;
-                    }
-                    top.offer(marks ? v : kNegInf, lead + at * V + e, k, bound, lane);
-                    marks &= marks - 1;
-                }
-            }
+            for (int e = 0; e < V2; ++e) y[e] = make_float2(kNegInf, kNegInf);
         }
-        if (WARPS == 1 || top.n > 32) top.keep(k, lane);
+        top.offer_pairs<V2>(y, [&](int e) { return lead + at * V + e; }, k, bound, lane);
     }
+}
 
-    if (WARPS > 1) {
-        if (lane == 0) {
-            sh.m[warp] = mo.m;
-            sh.s[warp] = mo.s;
-            sh.u[warp] = mo.u;
-            if constexpr (TOP) sh.n[warp] = top.n;
-        }
-        __syncthreads();
-        if constexpr (TOP) select_best(sh, WARPS, k);
-        cg::cluster_group cluster = cg::this_cluster();
-        if (parts > 1) {
-            cluster.sync();
-            if constexpr (TOP) {
-                if (part == 0) {
-                    // the peers' best k into this CTA's lists
-                    if (warp < parts) {
-                        const RowProbShared<TOP>* o = cluster.map_shared_rank(&sh, warp);
-                        const float v = lane < k ? o->ov[lane] : kNegInf;
-                        const int at = lane < k ? o->oi[lane] : -1;
-                        sh.lv[warp][lane] = v;
-                        sh.li[warp][lane] = at;
-                        const int have = __popc(__ballot_sync(0xffffffffu, at >= 0));
-                        if (lane == 0) sh.n[warp] = have;
-                    }
-                    __syncthreads();
-                    select_best(sh, parts, k);
-                }
-            }
-        }
-        if (part == 0 && warp == 0) {
-            // up to 8 x 8 parts, two to a lane
-            mo = Moments();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = (lane + 32 * h) / WARPS, w = lane % WARPS;
-                if (r < parts) {
-                    const RowProbShared<TOP>* o =
-                        parts > 1 ? cluster.map_shared_rank(&sh, r) : &sh;
-                    mo.merge(o->m[w], o->s[w], o->u[w], k2);
-                }
-            }
-            mo.join(k2);
-        }
-        if (parts > 1) cluster.sync();  // rank 0 has read this CTA's shared memory
-        if (part != 0 || warp != 0) return;
-    }
-
+// A finished row's outputs, by one warp; its best columns are lv / li [k].
+template <typename T, int SHAPE, bool TOP>
+__device__ __forceinline__ void write_row(const RowProbArgs& A, int64_t row, const T* X,
+                                          const RowShape& rs, const Moments& mo, const float* lv,
+                                          const int* li, int have, int lane) {
     // an empty row keeps s = 0; a row of NaN alone has s = NaN
     const bool none = mo.m == kNegInf && mo.s == 0.f;
     const float logs = none ? 0.f : logf(mo.s);
@@ -667,54 +587,584 @@ __global__ void __launch_bounds__(256, SHAPE ? 3 : 4) k_row_probs(const RowProbA
             A.logprob[row] = lp;
         }
     }
-    if constexpr (TOP) {
-        if (lane < k) {
-            const float* lv = WARPS == 1 ? top.v : sh.ov;
-            const int* li = WARPS == 1 ? top.i : sh.oi;
-            const bool held = WARPS == 1 ? lane < top.n : li[lane] >= 0;
-            A.top_lp[row * k + lane] = held ? fmaf(lv[lane] - mo.m, A.k, -logs) : kNegInf;
-            A.top_idx[row * k + lane] = held ? li[lane] : -1;
-        }
+    if (TOP && lane < A.top_k) {
+        const bool held = lane < have && li[lane] >= 0;
+        A.top_lp[row * A.top_k + lane] = held ? fmaf(lv[lane] - mo.m, A.k, -logs) : kNegInf;
+        A.top_idx[row * A.top_k + lane] = held ? li[lane] : -1;
     }
 }
 
-template <typename T, int SHAPE, bool TOP, int WARPS, int U>
-int launch_rows(const RowProbArgs& A, int cluster, cudaStream_t s) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    const int64_t ctas = WARPS == 1 ? (A.rows + 7) / 8 : A.rows * cluster;
-    if (ctas > INT_MAX) return fail(SK_ERR_ARG, "B * N is too large");
-    cfg.gridDim = dim3((unsigned)ctas);
-    if (WARPS > 1) {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = cluster;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
+// The row's ends, one column to a lane: up to V - 1 before the first whole
+// vector and as many behind the last.
+template <typename T, int SHAPE>
+__device__ __forceinline__ float row_ends(const T* X, const RowShape& rs, int lead, int tail,
+                                          int M, int lane, int& column) {
+    column = lane < 16 ? lane : tail + lane - 16;
+    const bool on = lane < 16 ? lane < lead : column < M;
+    return on ? shaped<SHAPE>(widen(X[column]), rs, column) : kNegInf;
+}
+
+// Short rows: a warp to a row, which is at most U vectors of 16 bytes a lane,
+// loaded at once and held in registers.
+template <typename T, int SHAPE, bool TOP, int U>
+__global__ void __launch_bounds__(32 * kRowWarps, U == 1 ? 4 : 3)
+    k_row_held(const RowProbArgs A) {
+    constexpr int V = Vec<T>::n, V2 = V / 2;
+    constexpr int H = U == 1 ? 1 : 16 / V;  // vectors folded at once: 16 values
+    static_assert(U % H == 0, "whole folds");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ RowStash<TOP> stash;
+    __shared__ RowShared<TOP, 1> shared[kRowWarps];
+    RowShared<TOP, 1>& sh = shared[warp];
+    const unsigned item = blockIdx.x / A.groups;  // (64-bit divisions cost as much as a row)
+    const int64_t b = item, r0 = (int64_t)(blockIdx.x - item * A.groups) * A.per_cta;
+    const T* const Xb = reinterpret_cast<const T*>(A.X) + b * A.sXb;
+    const int M = (int)A.M, k = A.top_k;
+    const float k2 = A.k * kLog2e;
+    const int64_t r1 = min(A.N, r0 + A.per_cta);
+    const T* X = nullptr;
+    int lead = 0, nv = 0;
+    uint4 raw[U];
+    auto load = [&](int64_t r) {
+        X = Xb + r * A.sXn;
+        lead = (int)row_lead(X, A.M);
+        nv = A.mask_a && !A.mask_a[b * A.N + r] ? 0 : (M - lead) / V;
+        const uint4* const body = reinterpret_cast<const uint4*>(X + lead);
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+            if (lane + q * 32 < nv) raw[q] = ld_stream16(body + lane + q * 32);
+    };
+    if (r0 + warp < r1) load(r0 + warp);
+    if (SHAPE != kPlain && A.staged) stage_g(A, b, 32 * kRowWarps);
+
+    for (int64_t r = r0 + warp; r < r1; r += kRowWarps) {
+        if (r != r0 + warp) load(r);
+        const int64_t row = b * A.N + r;
+        const bool masked_row = A.mask_a && !A.mask_a[row];
+        const RowShape rs = row_shape(A.g, A.sign, b, A.M, lead, A.staged);
+        const int tail = lead + nv * V;
+        float end = kNegInf;
+        int end_j = 0;
+        if (!masked_row && (lead > 0 || tail < M))
+            end = row_ends<T, SHAPE>(X, rs, lead, tail, M, lane, end_j);
+
+        Moments mo;
+        float high[U];  // largest value of each vector
+#pragma unroll
+        for (int h = 0; h < U; h += H) {
+            float2 x[H * V2];
+            float cm = kNegInf;
+#pragma unroll
+            for (int q = 0; q < H; ++q) {
+                const int at = lane + (h + q) * 32;
+                float2* const y = x + q * V2;
+                unpack2(raw[h + q], y, X);
+                if (at < nv) {
+                    shape_pairs<SHAPE, V2>(y, rs, lead + (int64_t)at * V);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V2; ++e) y[e] = make_float2(kNegInf, kNegInf);
+                }
+                float vm = fmaxf(y[0].x, y[0].y);
+#pragma unroll
+                for (int e = 1; e < V2; ++e) vm = fmaxf(vm, fmaxf(y[e].x, y[e].y));
+                high[h + q] = vm;
+                cm = fmaxf(cm, vm);
+            }
+            mo.fold<SHAPE != kPlain>(x, cm, k2);
+        }
+        if (!masked_row && (lead > 0 || tail < M)) {
+            const float2 e[1] = {make_float2(end, kNegInf)};
+            mo.fold<true>(e, end, k2);
+        }
+        mo.join(k2);
+
+        TopList top;
+        if constexpr (TOP) {
+            top.v = sh.lv[0];
+            top.i = sh.li[0];
+            if (lead > 0 || tail < M) top.offer(end, end_j, k, kNegInf, lane);
+            float best = kNegInf;
+#pragma unroll
+            for (int q = 0; q < U; ++q) best = fmaxf(best, high[q]);
+            const float bound = fmaxf(warp_rth_largest(best, k, lane), -FLT_MAX);
+            // vectors with a candidate to shared memory, then a value to a lane
+            if (lane == 0) stash.n[warp] = 0;
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < U; ++q)
+                if (high[q] >= bound) {
+                    const int at = atomicAdd(&stash.n[warp], 1);
+                    if (at < kStash) {
+                        stash.v[warp][at] = raw[q];
+                        stash.at[warp][at] = lane + q * 32;
+                    }
+                }
+            __syncwarp();
+            const int have = stash.n[warp];
+            if (have <= kStash) {
+                for (int c = 0; c < have * V; c += 32) {
+                    float v = kNegInf;
+                    int j = 0;
+                    if (c + lane < have * V) {
+                        const int q = (c + lane) / V, e = (c + lane) % V;
+                        j = lead + stash.at[warp][q] * V + e;
+                        v = shaped<SHAPE>(
+                            widen(reinterpret_cast<const T*>(&stash.v[warp][q])[e]), rs, j);
+                    }
+                    top.offer(v, j, k, bound, lane);
+                }
+            } else {  // many equal values
+                offer_again<T, SHAPE, U>(top, sh.from[0], best, bound, X, rs, lead, nv, 0,
+                                         32 * U, k, lane);
+            }
+            top.keep(k, lane);
+        }
+        write_row<T, SHAPE, TOP>(A, row, X, rs, mo, top.v, top.i, top.n, lane);
+        __syncwarp();  // the list is read
     }
-    SK_CUDA(cudaLaunchKernelEx(&cfg, k_row_probs<T, SHAPE, TOP, WARPS, U>, A));
+}
+
+// Long rows: a CTA of 8 warps to a row, or a cluster of CTAs where there are few
+// rows, joined over distributed shared memory by rank 0. As a step's vectors are
+// unpacked the loads of the next one take their registers.
+template <typename T, int SHAPE, bool TOP>
+__global__ void __launch_bounds__(32 * kRowWarps, SHAPE ? 3 : 4)
+    k_row_cta(const RowProbArgs A) {
+    constexpr int V = Vec<T>::n, V2 = V / 2, U = 4;
+    constexpr int H = 16 / V;  // vectors folded at once: 16 values
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ RowShared<TOP, kRowWarps> sh;
+    const int parts = (int)cg::this_cluster().num_blocks();
+    const int part = (int)cg::this_cluster().block_rank();
+    const unsigned of_all = blockIdx.x / (unsigned)parts, item = of_all / (unsigned)A.N;
+    const int64_t row = of_all, b = item, n = of_all - item * (unsigned)A.N;
+    const T* const X = reinterpret_cast<const T*>(A.X) + b * A.sXb + n * A.sXn;
+    const int M = (int)A.M, k = A.top_k;
+    const int lead = (int)row_lead(X, A.M);
+    const float k2 = A.k * kLog2e;
+    const bool masked_row = A.mask_a && !A.mask_a[row];
+    const int nv = masked_row ? 0 : (M - lead) / V;
+    const int wid = part * kRowWarps + warp, step = parts * kRowWarps * 32 * U;
+    const int base = wid * 32 * U + lane;
+    const uint4* const body = reinterpret_cast<const uint4*>(X + lead);
+    if (SHAPE != kPlain && A.staged) stage_g(A, b, 32 * kRowWarps);
+    const RowShape rs = row_shape(A.g, A.sign, b, A.M, lead, A.staged);
+    auto sync = [] { __syncthreads(); };
+
+    Moments mo;
+    float best = kNegInf;  // the lane's largest value among whole vectors
+    float2 x[H * V2];
+    auto fold = [&] {
+        float cm = kNegInf;
+#pragma unroll
+        for (int e = 0; e < H * V2; ++e) cm = fmaxf(cm, fmaxf(x[e].x, x[e].y));
+        if (TOP) best = fmaxf(best, cm);
+        mo.fold<SHAPE != kPlain>(x, cm, k2);
+    };
+    int i = base;
+    if (wid * 32 * U + 32 * U <= nv) {
+        uint4 raw[U];
+#pragma unroll
+        for (int q = 0; q < U; ++q) raw[q] = ld_stream16(body + i + q * 32);
+        const int last = nv - (32 * U - lane);  // of the steps that are whole
+        while (true) {
+            const bool more = i + step <= last;
+#pragma unroll
+            for (int h = 0; h < U; h += H) {
+#pragma unroll
+                for (int q = 0; q < H; ++q) {
+                    unpack2(raw[h + q], x + q * V2, X);
+                    if (more) raw[h + q] = ld_stream16(body + i + step + (h + q) * 32);
+                    shape_pairs<SHAPE, V2>(x + q * V2, rs,
+                                           lead + (int64_t)(i + (h + q) * 32) * V);
+                }
+                fold();
+            }
+            i += step;
+            if (!more) break;
+        }
+    }
+    for (; i - lane < nv; i += step) {  // the warp's last step
+#pragma unroll
+        for (int h = 0; h < U; h += H) {
+#pragma unroll
+            for (int q = 0; q < H; ++q) {
+                const int at = i + (h + q) * 32;
+                float2* const y = x + q * V2;
+                if (at < nv) {
+                    unpack2(ld_stream16(body + at), y, X);
+                    shape_pairs<SHAPE, V2>(y, rs, lead + (int64_t)at * V);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V2; ++e) y[e] = make_float2(kNegInf, kNegInf);
+                }
+            }
+            fold();
+        }
+    }
+    const int tail = lead + nv * V;
+    float end = kNegInf;
+    int end_j = 0;
+    if (!masked_row && wid == 0 && (lead > 0 || tail < M)) {
+        end = row_ends<T, SHAPE>(X, rs, lead, tail, M, lane, end_j);
+        const float2 e[1] = {make_float2(end, kNegInf)};
+        mo.fold<true>(e, end, k2);
+    }
+    mo.join(k2);
+    if (lane == 0) {
+        sh.m[warp] = mo.m;
+        sh.s[warp] = mo.s;
+        sh.u[warp] = mo.u;
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    const float* lv = nullptr;
+    const int* li = nullptr;
+    if constexpr (TOP) {
+        TopList top;
+        top.v = sh.lv[warp];
+        top.i = sh.li[warp];
+        top.offer(end, end_j, k, kNegInf, lane);
+        const float bound = lane_bound<kRowWarps>(sh, best, k, warp, lane, sync);
+        offer_again<T, SHAPE, U>(top, sh.from[warp], best, bound, X, rs, lead, nv, wid * 32 * U,
+                                 step, k, lane);
+        if (top.n > 32) top.keep(k, lane);
+        if (lane == 0) sh.n[warp] = top.n;
+        __syncthreads();
+        select_best<kRowWarps>(sh, kRowWarps, k, warp, lane, sync);
+        if (parts > 1) {
+            cluster.sync();
+            if (part == 0) {
+                // the peers' best k into this CTA's lists
+                if (warp < parts) {
+                    const auto* o = cluster.map_shared_rank(&sh, warp);
+                    const float v = lane < k ? o->ov[lane] : kNegInf;
+                    const int at = lane < k ? o->oi[lane] : -1;
+                    sh.lv[warp][lane] = v;
+                    sh.li[warp][lane] = at;
+                    const int have = __popc(__ballot_sync(0xffffffffu, at >= 0));
+                    if (lane == 0) sh.n[warp] = have;
+                }
+                __syncthreads();
+                select_best<kRowWarps>(sh, parts, k, warp, lane, sync);
+            }
+        }
+        lv = sh.ov;
+        li = sh.oi;
+    } else {
+        if (parts > 1) cluster.sync();
+        else __syncthreads();
+    }
+    if (part == 0 && warp == 0) {
+        // up to 8 x 8 parts, two to a lane
+        mo = Moments();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int q = (lane + 32 * h) / kRowWarps, w = lane % kRowWarps;
+            if (q < parts) {
+                const auto* o = parts > 1 ? cluster.map_shared_rank(&sh, q) : &sh;
+                mo.merge(o->m[w], o->s[w], o->u[w], k2);
+            }
+        }
+        mo.join(k2);
+        write_row<T, SHAPE, TOP>(A, row, X, rs, mo, lv, li, k, lane);
+    }
+    if (parts > 1) cluster.sync();  // rank 0 has read this CTA's shared memory
+}
+
+// Many rows: one CTA of up to 24 warps to an SM, each warp with a ring of 4 KB
+// stages of its own that bulk copies fill, so that the copies of the rows to come go on
+// while a row is joined and its best columns are found. TEAM warps share a row (1
+// up to 8 KB, else 4), and the CTA's teams a run of consecutive rows, item by
+// item; g stays in shared memory for an item.
+constexpr int kRingStages = 4;  // at most
+constexpr int kRingVecs = 8;    // vectors of a lane in a stage
+constexpr int kRingBytes = 32 * kRingVecs * 16;
+// Warps of a CTA. Without g 20 of them with 96 registers beat 24 with 80 (16384 x
+// 4096 bf16: 37 us against 51 us), with g it is the other way (16 x 2048 x 2048
+// with a mask and top 4: 101 us against 93 us).
+template <int SHAPE>
+constexpr int ring_warps() {
+    return SHAPE == kPlain ? 20 : 24;
+}
+
+template <typename T, int SHAPE, bool TOP, int TEAM>
+__global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const RowProbArgs A) {
+    constexpr int V = Vec<T>::n, V2 = V / 2;
+    constexpr int H = 32 / V < kRingVecs ? 32 / V : kRingVecs;  // vectors folded at once
+    constexpr int WARPS = ring_warps<SHAPE>(), TEAMS = WARPS / TEAM;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int team = warp / TEAM, tw = warp % TEAM;
+    __shared__ RowShared<TOP, TEAM> shared[TEAMS];
+    __shared__ uint64_t bars[WARPS][kRingStages];
+    RowShared<TOP, TEAM>& sh = shared[team];
+    uint64_t* const full = bars[warp];
+    const int stages = A.stages;
+    uint8_t* const ring = reinterpret_cast<uint8_t*>(staged_g) +
+                          (A.staged ? align16((int)A.M * 4) : 0) + warp * stages * kRingBytes;
+    auto sync = [&] {
+        if (TEAM == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(TEAM * 32) : "memory");
+    };
+    if (lane == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+        mbar_init_fence();
+    }
+    __syncwarp();
+
+    const int64_t rows = A.B * A.N;  // below 2^31
+    const int R0 = (int)(rows * blockIdx.x / gridDim.x);
+    const int R1 = (int)(rows * (blockIdx.x + 1) / gridDim.x);
+    const unsigned N = (unsigned)A.N;
+    const int M = (int)A.M, k = A.top_k;
+    const float k2 = A.k * kLog2e;
+    const int first = tw * 32 * kRingVecs, step = TEAM * 32 * kRingVecs;
+    // without g the CTA's rows are one run; with it, runs of an item
+    auto run_end = [&](int r) {
+        return SHAPE == kPlain ? R1 : (int)min((unsigned)R1, (r / N + 1) * N);
+    };
+    // a team's rows: of each run the team-th, and every TEAMS-th from there
+    auto next_row = [&](int r, int& end) {
+        r += TEAMS;
+        while (r >= end && end < R1) {
+            r = end + team;
+            end = run_end(end);
+        }
+        return r;
+    };
+    // The copies: the row they are at, where this warp's next step of it lies and
+    // how many vectors the row has from there on.
+    int ahead_end = run_end(R0), ahead = next_row(R0 + team - TEAMS, ahead_end);
+    const T* src = nullptr;
+    int left = 0;
+    auto open = [&](unsigned row) {
+        const unsigned b = row / N;
+        const T* const X =
+            reinterpret_cast<const T*>(A.X) + b * A.sXb + (int64_t)(row - b * N) * A.sXn;
+        const int lead = (int)row_lead(X, A.M);
+        src = X + lead + first * V;
+        left = A.mask_a && !A.mask_a[row] ? 0 : (M - lead) / V - first;
+    };
+    if (ahead < R1) open(ahead);
+    int issue_at = 0, use_at = 0;  // stages
+    uint32_t phase = 0;            // bit s: the phase to wait for
+    // the copy of the next step into the stage that is free
+    auto issue = [&] {
+        while (left <= 0) {
+            if (ahead < R1) ahead = next_row(ahead, ahead_end);
+            if (ahead >= R1) return;
+            open(ahead);
+        }
+        if (lane == 0) {
+            const uint32_t bytes = min(32 * kRingVecs, left) * 16;
+            mbar_expect_tx(&full[issue_at], bytes);
+            bulk_g2s(ring + issue_at * kRingBytes, src, bytes, &full[issue_at]);
+        }
+        if (++issue_at == stages) issue_at = 0;
+        src += step * V;
+        left -= step;
+    };
+    for (int s = 0; s < stages; ++s) issue();
+
+    bool ok = true;
+    int end = run_end(R0);
+    for (int run = R0; run < R1; run = end, end = run_end(run)) {
+        const unsigned item0 = SHAPE == kPlain ? 0 : run / N;
+        if (SHAPE != kPlain && A.staged) {
+            __syncthreads();  // the last item's g is read
+            stage_g(A, item0, WARPS * 32);
+        }
+        for (int row = run + team; row < end; row += TEAMS) {
+            const unsigned b = SHAPE == kPlain ? row / N : item0;
+            const int64_t n = row - b * N;
+            const T* const X = reinterpret_cast<const T*>(A.X) + b * A.sXb + n * A.sXn;
+            const int lead = (int)row_lead(X, A.M);
+            const RowShape rs = row_shape(A.g, A.sign, b, A.M, lead, A.staged);
+            const bool masked_row = A.mask_a && !A.mask_a[row];
+            const int nv = masked_row ? 0 : (M - lead) / V;
+            Moments mo;
+            float best = kNegInf;
+            for (int i = first; i < nv; i += step) {
+                if (!mbar_try_wait(&full[use_at], phase >> use_at & 1))
+                    ok = mbar_wait(&full[use_at], phase >> use_at & 1) && ok;
+                __syncwarp();
+                phase ^= 1u << use_at;
+                const uint4* const p =
+                    reinterpret_cast<const uint4*>(ring + use_at * kRingBytes) + lane;
+                if (++use_at == stages) use_at = 0;
+                const bool whole = i + 32 * kRingVecs <= nv;
+#pragma unroll
+                for (int h = 0; h < kRingVecs; h += H) {
+                    uint4 raw[H];
+#pragma unroll
+                    for (int q = 0; q < H; ++q) raw[q] = p[(h + q) * 32];
+                    if (h + H == kRingVecs) {
+                        __syncwarp();  // the stage is read
+                        issue();
+                    }
+                    float2 x[H * V2];
+                    float cm = kNegInf;
+#pragma unroll
+                    for (int q = 0; q < H; ++q) {
+                        const int at = i + (h + q) * 32 + lane;
+                        float2* const y = x + q * V2;
+                        unpack2(raw[q], y, X);
+                        if (whole || at < nv) {
+                            shape_pairs<SHAPE, V2>(y, rs, lead + (int64_t)at * V);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < V2; ++e) y[e] = make_float2(kNegInf, kNegInf);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < H * V2; ++e) cm = fmaxf(cm, fmaxf(x[e].x, x[e].y));
+                    if (TOP) best = fmaxf(best, cm);
+                    mo.fold<SHAPE != kPlain>(x, cm, k2);
+                }
+            }
+            const int tail = lead + nv * V;
+            float endv = kNegInf;
+            int end_j = 0;
+            if (!masked_row && tw == 0 && (lead > 0 || tail < M)) {
+                endv = row_ends<T, SHAPE>(X, rs, lead, tail, M, lane, end_j);
+                const float2 e[1] = {make_float2(endv, kNegInf)};
+                mo.fold<true>(e, endv, k2);
+            }
+            mo.join(k2);
+            if (__any_sync(0xffffffffu, !ok)) mo.s = NAN;  // a copy never came: the row says so
+
+            TopList top;
+            if constexpr (TOP) {
+                top.v = sh.lv[tw];
+                top.i = sh.li[tw];
+                top.offer(endv, end_j, k, kNegInf, lane);
+                const float bound = lane_bound<TEAM>(sh, best, k, tw, lane, sync);
+                offer_again<T, SHAPE, kRingVecs>(top, sh.from[tw], best, bound, X, rs,
+                                                 lead, nv, first, step, k, lane);
+                if (TEAM == 1 || top.n > 32) top.keep(k, lane);
+            }
+            if constexpr (TEAM == 1) {
+                write_row<T, SHAPE, TOP>(A, row, X, rs, mo, top.v, top.i, top.n, lane);
+                __syncwarp();
+            } else {
+                if (lane == 0) {
+                    sh.m[tw] = mo.m;
+                    sh.s[tw] = mo.s;
+                    sh.u[tw] = mo.u;
+                    if constexpr (TOP) sh.n[tw] = top.n;
+                }
+                sync();
+                if constexpr (TOP) select_best<TEAM>(sh, TEAM, k, tw, lane, sync);
+                if (tw == 0) {
+                    mo = Moments();
+                    if (lane < TEAM) mo.merge(sh.m[lane], sh.s[lane], sh.u[lane], k2);
+                    mo.join(k2);
+                    const float* lv = nullptr;
+                    const int* li = nullptr;
+                    if constexpr (TOP) {
+                        lv = sh.ov;
+                        li = sh.oi;
+                    }
+                    write_row<T, SHAPE, TOP>(A, row, X, rs, mo, lv, li, k, lane);
+                }
+                sync();  // what the team shares of this row is read
+            }
+        }
+    }
+    // copies that a wait gave up on may still be on their way
+    if (!ok)
+        for (int s = 0; s < stages; ++s) mbar_wait(&full[s], phase >> s & 1, 1u << 12);
+}
+
+constexpr int64_t kStagedMax = 16384;  // columns of g that are held in shared memory
+
+// Shared memory of a kernel that holds an item's g beside its own: `held` is 0
+// where g is not staged.
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+    if (bytes > 16384)
+        SK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)bytes));
     return SK_OK;
 }
 
-// How a row is split. A warp per row needs no join, and serves short rows and
-// row counts that fill the SMs with warps; longer or fewer rows take a CTA, and
-// where the rows alone leave SMs idle a cluster of up to 8 CTAs (each with at
-// least one full step of its 8 warps).
+template <typename T, int SHAPE, bool TOP, int U>
+int launch_held(RowProbArgs A, int per_cta, cudaStream_t s) {
+    A.per_cta = per_cta;
+    // a row of one vector a lane waits longer for the CTA's g than for its own from L1
+    if (U == 1 && !A.mask_b) A.staged = false;
+    A.groups = (unsigned)((A.N + per_cta - 1) / per_cta);
+    const int64_t ctas = A.groups * A.B;
+    if (ctas > INT_MAX) return fail(SK_ERR_ARG, "B * N is too large");
+    const size_t smem = A.staged ? align16((int)A.M * 4) : 0;  // at most 4 KB
+    k_row_held<T, SHAPE, TOP, U><<<(unsigned)ctas, 32 * kRowWarps, smem, s>>>(A);
+    SK_LAUNCHED("k_row_held");
+    return SK_OK;
+}
+
+template <typename T, int SHAPE, bool TOP>
+int launch_cta(const RowProbArgs& A, int cluster, cudaStream_t s) {
+    const int64_t ctas = A.B * A.N * cluster;
+    if (ctas > INT_MAX) return fail(SK_ERR_ARG, "B * N is too large");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(32 * kRowWarps);
+    cfg.dynamicSmemBytes = A.staged ? align16((int)A.M * 4) : 0;
+    cfg.stream = s;
+    const int rc = allow_smem(k_row_cta<T, SHAPE, TOP>, cfg.dynamicSmemBytes);
+    if (rc != SK_OK) return rc;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    SK_CUDA(cudaLaunchKernelEx(&cfg, k_row_cta<T, SHAPE, TOP>, A));
+    return SK_OK;
+}
+
+template <typename T, int SHAPE, bool TOP, int TEAM>
+int launch_ring(RowProbArgs A, cudaStream_t s) {
+    cudaFuncAttributes fa;
+    SK_CUDA(cudaFuncGetAttributes(&fa, k_row_ring<T, SHAPE, TOP, TEAM>));
+    const size_t held = A.staged ? align16((int)A.M * 4) : 0;
+    const size_t stage = (size_t)ring_warps<SHAPE>() * kRingBytes;
+    A.stages = (int)std::min<size_t>(kRingStages, (232448 - fa.sharedSizeBytes - held) / stage);
+    const size_t smem = held + A.stages * stage;
+    const int rc = allow_smem(k_row_ring<T, SHAPE, TOP, TEAM>, smem);
+    if (rc != SK_OK) return rc;
+    const int64_t rows = A.B * A.N, teams = ring_warps<SHAPE>() / TEAM;
+    const unsigned grid = (unsigned)std::min<int64_t>(148, (rows + teams - 1) / teams);
+    k_row_ring<T, SHAPE, TOP, TEAM><<<grid, ring_warps<SHAPE>() * 32, smem, s>>>(A);
+    SK_LAUNCHED("k_row_ring");
+    return SK_OK;
+}
+
+// How the rows are split. Up to 2 KB a warp holds a row in registers and nothing
+// is joined or read twice; a CTA takes at least a row of an item to each warp.
+// Longer rows go to the rings where there are enough to keep them busy (and, with
+// a g that is staged per item, items of some length), else a row takes a CTA, or
+// a cluster of up to 8 where the rows alone leave SMs idle (each with at least
+// one full step of its warps).
 template <typename T, int SHAPE, bool TOP>
 int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
-    constexpr int U = 4;
-    const int64_t bytes = A.M * (int64_t)sizeof(T);
-    if (bytes <= 512) return launch_rows<T, SHAPE, TOP, 1, 1>(A, 1, s);
-    if (bytes <= 2048 || (bytes <= 16384 && A.rows >= 148 * 16))
-        return launch_rows<T, SHAPE, TOP, 1, U>(A, 1, s);
+    const int64_t bytes = A.M * (int64_t)sizeof(T), rows = A.B * A.N;
+    if (bytes <= 2048) {
+        const int64_t want = rows / (148 * 24) / kRowWarps * kRowWarps;
+        const int per = (int)std::max<int64_t>(kRowWarps, std::min<int64_t>(want, 32));
+        return bytes <= 512 ? launch_held<T, SHAPE, TOP, 1>(A, per, s)
+                            : launch_held<T, SHAPE, TOP, 4>(A, per, s);
+    }
+    const bool runs = (SHAPE == kPlain || A.N >= 64) && rows < INT_MAX / 2;
+    if (bytes <= 8192 && rows >= 148 * 16 && runs) return launch_ring<T, SHAPE, TOP, 1>(A, s);
+    if (SHAPE != kPlain && bytes > 8192 && rows >= 148 * 4 && runs)
+        return launch_ring<T, SHAPE, TOP, 4>(A, s);
     int cluster = 1;
-    while (cluster < 8 && A.rows * cluster * 2 <= 148 * 4 &&
-           bytes > (int64_t)cluster * kRowWarps * 32 * U * 16)
+    while (cluster < 8 && rows * cluster * 2 <= 148 * 4 &&
+           bytes > (int64_t)cluster * kRowWarps * 32 * 4 * 16)
         cluster *= 2;
-    return launch_rows<T, SHAPE, TOP, kRowWarps, U>(A, cluster, s);
+    return launch_cta<T, SHAPE, TOP>(A, cluster, s);
 }
 
 template <typename T, int SHAPE>
@@ -1118,7 +1568,7 @@ int check_rows(const void* X, int dtype, int64_t B, int64_t N, int64_t M, int64_
 extern "C" {
 
 size_t sk_row_logprobs_workspace_bytes(int64_t B, int64_t M) {
-    if (B <= 0 || M <= 0) return 0;
+    if (B <= 0 || M <= sk::kStagedMax) return 0;
     return sk::align_up(sizeof(float) * (size_t)B * M);
 }
 
@@ -1136,18 +1586,24 @@ int sk_row_logprobs(const void* X, int dtype, int64_t B, int64_t N, int64_t M, i
         return fail(SK_ERR_ARG, "targets and logprob go together");
     if (top_k > 0 && (!top_logprob || !top_index))
         return fail(SK_ERR_ARG, "top_k needs top_logprob and top_index");
-    if (mask_b && (!workspace || workspace_bytes < sk_row_logprobs_workspace_bytes(B, M)))
+    if (mask_b && M > kStagedMax &&
+        (!workspace || workspace_bytes < sk_row_logprobs_workspace_bytes(B, M)))
         return fail(SK_ERR_WORKSPACE, "workspace too small for sk_row_logprobs with mask_b");
     cudaStream_t s = (cudaStream_t)stream;
-    const int fm = fold_mask(&g, mask_b, B * M, workspace, s);
-    if (fm != SK_OK) return fm;
     RowProbArgs A{};
+    A.staged = (g || mask_b) && M <= kStagedMax;
+    if (A.staged) {
+        A.mask_b = mask_b;
+    } else {
+        const int fm = fold_mask(&g, mask_b, B * M, workspace, s);
+        if (fm != SK_OK) return fm;
+    }
     A.X = X;
     A.N = N;
     A.M = M;
     A.sXb = sXb;
     A.sXn = sXn;
-    A.rows = B * N;
+    A.B = B;
     A.g = g;
     A.mask_a = mask_a;
     A.sign = negate ? -1.f : 1.f;
@@ -1173,7 +1629,8 @@ size_t sk_row_logprobs_backward_workspace_bytes(int64_t B, int64_t N, int64_t M)
         sk::bwd_bands(B, N, M, true, elem, &nb, &br);
         most = std::max(most, nb);
     }
-    return sk_row_logprobs_workspace_bytes(B, M) + sk::align_up(sizeof(float) * (size_t)B * most * M);
+    return sk::align_up(sizeof(float) * (size_t)B * M) +
+           sk::align_up(sizeof(float) * (size_t)B * most * M);
 }
 
 int sk_row_logprobs_backward(const void* X, int dtype, int64_t B, int64_t N, int64_t M,
@@ -1221,7 +1678,7 @@ int sk_row_logprobs_backward(const void* X, int dtype, int64_t B, int64_t N, int
     A.g_ent = grad_entropy;
     A.g_top = grad_top;
     A.dX = dX;
-    if (dg) A.partial = (float*)((char*)workspace + sk_row_logprobs_workspace_bytes(B, M));
+    if (dg) A.partial = (float*)((char*)workspace + align_up(sizeof(float) * (size_t)B * M));
     bwd_bands(B, N, M, dg != nullptr, dtype == SK_FP32 ? 4 : 2, &A.bands, &A.band_rows);
     const bool masked = mask_b != nullptr;
     if (dtype == SK_FP32) return launch_bwd_typed<float>(A, masked, dg, s);
