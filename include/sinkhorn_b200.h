@@ -559,7 +559,8 @@ int sk_row_logprobs(const void* X, int dtype, int64_t B, int64_t N, int64_t M, i
                     int64_t* top_index, float* stats, void* workspace, size_t workspace_bytes,
                     void* stream);
 
-/* Workspace bytes of sk_row_logprobs (needed with mask_b only). */
+/* Workspace bytes of sk_row_logprobs (needed with mask_b only; 0 up to 16384
+ * columns). */
 size_t sk_row_logprobs_workspace_bytes(int64_t B, int64_t M);
 
 /* Workspace bytes of sk_row_logprobs_backward (needed with mask_b, and when dg

@@ -43,17 +43,11 @@ constexpr int kBandC = 8;    // column tiles that share a pass over the weights
 constexpr int kThreads = 192;  // producer warp, MMA warp, four epilogue warps
 constexpr int kMaxGroups = 1024;
 
-// BN: most columns of a tile. 256, or 64 for short groups, whose products are
-// bound by the read of the weights: a stage is then nearly all weights and more
-// of them are in flight.
-template <int BN>
-struct Shape {
-    static constexpr int kHalf = BN / 2;  // columns of B in each CTA
-    static constexpr int kStageBytes = kABytes + kHalf * kBK * 2;
-    static constexpr int kStages = BN == 256 ? 6 : 10;
-    static constexpr uint32_t kTmemCols = 2 * BN;  // two accumulators
-};
-constexpr int kMaxStages = 10;
+constexpr int kBN = 256;     // most columns of a tile
+constexpr int kHalf = kBN / 2;  // columns of B in each CTA
+constexpr int kStageBytes = kABytes + kHalf * kBK * 2;
+constexpr int kStages = 6;
+constexpr uint32_t kTmemCols = 2 * kBN;  // two accumulators
 
 struct GroupedArgs {
     CUtensorMap a, b, b32;  // b32: boxes of 32 columns, for narrow tiles
@@ -70,7 +64,7 @@ struct alignas(16) GroupedShared {
     // empty, acc_full: committed by the MMAs to both. A stage whose last rows are
     // cleared takes another way: the second CTA's copies complete on its own
     // `part`, and it signals the leading CTA's `ready` once they are cleared.
-    uint64_t full[kMaxStages], empty[kMaxStages], part[kMaxStages], ready[kMaxStages];
+    uint64_t full[kStages], empty[kStages], part[kStages], ready[kStages];
     uint64_t acc_full[2], acc_empty[2], drain;
     uint32_t tmem;
     int gave_up;  // a bounded wait ran out: the CTA's remaining tiles become NaN
@@ -122,9 +116,8 @@ __device__ __forceinline__ bool wait_peer_warp(GroupedShared* sh, uint64_t* bar,
     return __shfl_sync(0xffffffffu, (int)ok, 0);
 }
 
-template <int BN>
 __device__ __forceinline__ int column_tiles(int rows) {
-    return (rows + BN - 1) / BN;
+    return (rows + kBN - 1) / kBN;
 }
 
 // A role's place among the groups: its tiles only go up.
@@ -133,7 +126,6 @@ struct Walk {
 };
 
 // Tile t of the launch.
-template <int BN>
 __device__ __forceinline__ Tile tile_at(const GroupedArgs& A, const GroupedShared* sh, int t,
                                         Walk& walk) {
     Tile q;
@@ -143,7 +135,7 @@ __device__ __forceinline__ Tile tile_at(const GroupedArgs& A, const GroupedShare
         while (lo <= A.E && sh->tile0[lo + 1] <= t) ++lo;
         walk.group = lo;
         const int r0 = sh->first[lo], rows = sh->first[lo + 1] - r0;
-        const int nc = column_tiles<BN>(rows);
+        const int nc = column_tiles(rows);
         // even tiles, in bands that reuse what of the weights they have loaded
         const int each = ((rows + nc - 1) / nc + 31) / 32 * 32;
         int l = t - sh->tile0[lo];
@@ -158,15 +150,15 @@ __device__ __forceinline__ Tile tile_at(const GroupedArgs& A, const GroupedShare
         q.k0 = 0;
         q.depth = q.group >= 0 ? A.k : 0;
     } else {
-        const int nc = column_tiles<BN>(A.c);
+        const int nc = column_tiles(A.c);
         q.group = t / (nm * nc);
         int l = t - q.group * nm * nc;
         const int band = l / (kBandC * nm);
         l -= band * kBandC * nm;
         const int wide = min(kBandC, nc - band * kBandC);
         q.m0 = l / wide * kPairM;
-        q.c0 = (band * kBandC + l % wide) * BN;
-        q.cols = min(BN, A.c - q.c0);
+        q.c0 = (band * kBandC + l % wide) * kBN;
+        q.cols = min(kBN, A.c - q.c0);
         q.k0 = sh->first[q.group + 1];
         q.depth = sh->first[q.group + 2] - q.k0;
     }
@@ -188,7 +180,6 @@ __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
 
 // Group bounds and tile counts, by one warp. Offsets that fall or leave [0, S]
 // are brought back: no tile then reaches outside the rows.
-template <int BN>
 __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
     const int nm = (A.m + kPairM - 1) / kPairM;
     int reach = 0, tiles = 0;  // running maximum of the offsets, running tile count
@@ -205,7 +196,7 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
         o = max(o, reach);
         int before = __shfl_up_sync(0xffffffffu, o, 1);
         if (lane == 0) before = reach;
-        int n = i <= A.E + 1 ? column_tiles<BN>(o - before) * nm : 0;  // tiles of group i
+        int n = i <= A.E + 1 ? column_tiles(o - before) * nm : 0;  // tiles of group i
         int sum = n;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
@@ -219,7 +210,7 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
         reach = __shfl_sync(0xffffffffu, o, 31);
         tiles += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) sh->tiles = A.by_rows ? tiles : A.E * nm * column_tiles<BN>(A.c);
+    if (lane == 0) sh->tiles = A.by_rows ? tiles : A.E * nm * column_tiles(A.c);
 }
 
 // The accumulators to memory. D has the output's contiguous dimension on the
@@ -227,7 +218,7 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
 // fragments are stored transposed, and leave as 16-byte pieces of output rows, 8
 // rows of 64 bytes to an instruction. Outputs whose rows do not start on 16
 // bytes leave element by element.
-template <typename T, int BN>
+template <typename T>
 __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh, int rank,
                                          int quarter, int lane) {
     int used = 0;  // accumulators so far
@@ -241,7 +232,7 @@ __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh
                       (reinterpret_cast<uintptr_t>(A.out) & 15) == 0;
     Walk walk;
     for (int t = blockIdx.x / 2; t < sh->tiles; t += gridDim.x / 2) {
-        const Tile q = tile_at<BN>(A, sh, t, walk);
+        const Tile q = tile_at(A, sh, t, walk);
         const int m0 = q.m0 + rank * kBM + quarter * 32;  // the warp's lanes
         T* const out = reinterpret_cast<T*>(A.out) +
                        (A.by_rows ? 0 : q.group * A.out_group) + (int64_t)q.c0 * A.ldo + m0;
@@ -252,7 +243,7 @@ __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh
             tc_fence_after();
         }
         const bool held = q.depth > 0 && ok;
-        const uint32_t acc = sh->tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN;
+        const uint32_t acc = sh->tmem + ((uint32_t)(quarter * 32) << 16) + buf * kBN;
         const uint32_t fill = __float_as_uint(ok ? 0.f : NAN);
         if (wide) {
             // piece p = lane % 4 of rows lane / 4 + 8 i
@@ -365,24 +356,22 @@ __device__ __forceinline__ void clear_rows(uint8_t* stage, int n, int left, int 
     __syncwarp();
 }
 
-template <int BN>
 __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__ GroupedArgs A) {
-    using Z = Shape<BN>;
     extern __shared__ uint8_t dyn[];
     uint8_t* const stages =
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
     GroupedShared* const sh =
-        reinterpret_cast<GroupedShared*>(stages + Z::kStages * Z::kStageBytes);
+        reinterpret_cast<GroupedShared*>(stages + kStages * kStageBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_ctarank();
     const int t0 = blockIdx.x / 2, dt = gridDim.x / 2;  // the pair's tiles
 
     if (warp == 0) {
-        plan_groups<BN>(A, sh, lane);
+        plan_groups(A, sh, lane);
     } else if (warp == 1) {
-        tmem_alloc_pair(&sh->tmem, Z::kTmemCols);
+        tmem_alloc_pair(&sh->tmem, kTmemCols);
         if (lane == 0) {
-            for (int s = 0; s < Z::kStages; ++s) {
+            for (int s = 0; s < kStages; ++s) {
                 mbar_init(&sh->full[s], 1);
                 mbar_init(&sh->empty[s], 1);
                 mbar_init(&sh->part[s], 1);
@@ -412,21 +401,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
     // registers; they are stepped, and the next barrier is looked at before the
     // current stage is issued.
     if (warp == 0) {
-        Ring<Z::kStages> ring;
+        Ring<kStages> ring;
         const uint32_t full0 = map_to_rank(&sh->full[0], 0);  // the leading CTA's
         const uint32_t part0 = map_to_rank(&sh->part[0], 1);
         const bool leader = elect_one();
         bool ok = true;
         Walk walk;
         for (int t = t0; ok && t < sh->tiles; t += dt) {
-            const Tile q = tile_at<BN>(A, sh, t, walk);
+            const Tile q = tile_at(A, sh, t, walk);
             // this CTA's lanes and its half of the columns
             const int m0 = q.m0 + rank * kBM;
             const int half = (q.cols + 31) / 32 * 16, c0 = q.c0 + rank * half;
             // boxes of 64 columns (MN-major), of 32 or one of all (K-major)
             const bool narrow = !A.b_mn && half <= 64;
             const int boxes = A.b_mn ? (half + 63) / 64 : narrow ? (half + 31) / 32 : 1;
-            const int box = A.b_mn ? kBox : (narrow ? 32 : Z::kHalf) * kBK * 2;
+            const int box = A.b_mn ? kBox : (narrow ? 32 : kHalf) * kBK * 2;
             const int z = A.by_rows ? q.group : 0;
             const uint32_t bytes = kABytes + boxes * box;
             const CUtensorMap* const mb = narrow ? &A.b32 : &A.b;
@@ -436,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                 if (ring.lap) ok = wait_warp(sh, &sh->empty[ring.s], (ring.lap - 1) & 1);
                 if (!ok) break;
                 if (leader) {
-                    uint8_t* const sa = stages + ring.s * Z::kStageBytes;
+                    uint8_t* const sa = stages + ring.s * kStageBytes;
                     uint8_t* const sb = sa + kABytes;
                     const bool clear = cleared > 0 && k + kBK > end;
                     uint32_t bar = full0 + ring.s * 8;
@@ -471,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
             for (int i = 0; i < 1000; ++i) __nanosleep(1000);
         __syncwarp();
     } else if (warp == 1) {
-        Ring<Z::kStages> ring;
+        Ring<kStages> ring;
         uint32_t parts = 0;  // bit s: phase of part[s] / ready[s]
         int used = 0;
         bool ok = true;
@@ -484,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
         const uint32_t ja = (A.a_mn ? 2048 : 32) >> 4, jb = (A.b_mn ? 2048 : 32) >> 4;
         Walk walk;
         for (int t = t0; ok && t < sh->tiles; t += dt) {
-            const Tile q = tile_at<BN>(A, sh, t, walk);
+            const Tile q = tile_at(A, sh, t, walk);
             if (q.depth <= 0) continue;
             const int n = (q.cols + 31) / 32 * 32;
             const int blocks = (q.depth + kBK - 1) / kBK;
@@ -498,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                     ok = wait_warp(sh, &sh->part[st], parts >> st & 1);
                     if (!ok) break;
                     parts ^= 1u << st;
-                    clear_rows(stages + st * Z::kStageBytes, n, left, cleared, lane);
+                    clear_rows(stages + st * kStageBytes, n, left, cleared, lane);
                     if (lane == 0) mbar_arrive_cluster(map_to_rank(&sh->ready[st], 0));
                 }
                 ring.next();
@@ -507,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
             const int buf = used & 1;
             if (used >= 2) ok = wait_warp(sh, &sh->acc_empty[buf], (used / 2 - 1) & 1);
             if (!ok) break;
-            const uint32_t d = tmem + buf * BN;
+            const uint32_t d = tmem + buf * kBN;
             const uint32_t idesc = mma_idesc(A.bf16, A.a_mn, A.b_mn, kPairM, n);
             const int whole = left == kBK ? blocks : blocks - 1;
             bool seen = whole > 0 && mbar_try_wait(&sh->full[ring.s], ring.lap & 1);
@@ -520,8 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                 seen = i + 1 < whole && mbar_try_wait(&sh->full[ring.s], ring.lap & 1);
                 tc_fence_after();
                 if (leader) {
-                    const uint64_t da = da0 + st * (Z::kStageBytes >> 4);
-                    const uint64_t db = db0 + st * (Z::kStageBytes >> 4);
+                    const uint64_t da = da0 + st * (kStageBytes >> 4);
+                    const uint64_t db = db0 + st * (kStageBytes >> 4);
                     mma_f16_pair(d, da, db, idesc, i > 0);
                     mma_f16_pair(d, da + ja, db + jb, idesc, true);
                     mma_f16_pair(d, da + 2 * ja, db + 2 * jb, idesc, true);
@@ -536,15 +525,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
                 ok = wait_warp(sh, &sh->full[st], ring.lap & 1);
                 if (!ok) break;
                 if (cleared > 0) {
-                    clear_rows(stages + st * Z::kStageBytes, n, left, cleared, lane);
+                    clear_rows(stages + st * kStageBytes, n, left, cleared, lane);
                     ok = wait_peer_warp(sh, &sh->ready[st], parts >> st & 1, lane);
                     if (!ok) break;
                     parts ^= 1u << st;
                 }
                 tc_fence_after();
                 if (leader) {
-                    const uint64_t da = da0 + st * (Z::kStageBytes >> 4);
-                    const uint64_t db = db0 + st * (Z::kStageBytes >> 4);
+                    const uint64_t da = da0 + st * (kStageBytes >> 4);
+                    const uint64_t db = db0 + st * (kStageBytes >> 4);
                     for (int j = 0; j < (left + 15) / 16; ++j)
                         mma_f16_pair(d, da + j * ja, db + j * jb, idesc, whole + j > 0);
                     mma_commit_pair(&sh->empty[st]);
@@ -563,28 +552,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_grouped(const __grid_constant__
         }
         __syncwarp();
     } else {
-        if (A.bf16) epilogue<__nv_bfloat16, BN>(A, sh, rank, warp & 3, lane);
-        else epilogue<__half, BN>(A, sh, rank, warp & 3, lane);
+        if (A.bf16) epilogue<__nv_bfloat16>(A, sh, rank, warp & 3, lane);
+        else epilogue<__half>(A, sh, rank, warp & 3, lane);
     }
     tc_fence_before();
     __syncthreads();
     cluster_barrier();  // neither CTA reads or signals the other any more
     if (warp == 1) {
         tc_fence_after();
-        tmem_free_pair(sh->tmem, Z::kTmemCols);
+        tmem_free_pair(sh->tmem, kTmemCols);
     }
 }
 
 // dst[g][r][0..ld) = src: an operand whose rows do not start on 16 bytes, laid
-// out so that they do (ld is the width rounded up to 8 elements).
+// out so that they do (ld is the width rounded up to 8 elements, the padding 0).
+// Eight elements a thread, read one by one and written at once.
 __global__ void __launch_bounds__(256) k_grouped_pack(const uint16_t* src, int64_t sg, int64_t sr,
-                                                      int64_t rows, int64_t width, int64_t ld,
-                                                      int64_t total_rows, uint16_t* dst) {
-    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < total_rows;
-         r += (int64_t)gridDim.x * 8) {
-        const uint16_t* const s = src + r / rows * sg + r % rows * sr;
-        uint16_t* const d = dst + r * ld;
-        for (int64_t i = threadIdx.x & 31; i < width; i += 32) d[i] = s[i];
+                                                      unsigned rows, int width, unsigned pieces,
+                                                      int64_t total, uint4* dst) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+         i += (int64_t)gridDim.x * 256) {
+        const unsigned r = (unsigned)(i / pieces), x = (unsigned)(i - (int64_t)r * pieces) * 8;
+        const uint16_t* const s = src + (int64_t)(r / rows) * sg + (int64_t)(r % rows) * sr + x;
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (int)x + e < width ? s[e] : 0;
+        dst[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16,
+                            v[6] | v[7] << 16);
     }
 }
 
@@ -602,10 +596,10 @@ struct Operand {
     }
     int pack(char*& ws, cudaStream_t s) {
         if (ready()) return SK_OK;
-        const int64_t ld = (width + 7) / 8 * 8, total = groups * rows;
-        const unsigned grid = (unsigned)std::min<int64_t>((total + 7) / 8, 148 * 16);
-        k_grouped_pack<<<grid, 256, 0, s>>>((const uint16_t*)p, sg, sr, rows, width, ld, total,
-                                            (uint16_t*)ws);
+        const int64_t ld = (width + 7) / 8 * 8, total = groups * rows * (ld / 8);
+        const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 32);
+        k_grouped_pack<<<grid, 256, 0, s>>>((const uint16_t*)p, sg, sr, (unsigned)rows,
+                                            (int)width, (unsigned)(ld / 8), total, (uint4*)ws);
         SK_LAUNCHED("k_grouped_pack");
         const size_t used = packed_bytes();
         p = ws;
@@ -655,15 +649,9 @@ int encode(CUtensorMap* map, const Operand& o, bool bf16, uint32_t box_rows) {
     return SK_OK;
 }
 
-template <int BN>
-constexpr size_t grouped_smem() {
-    return 1024 + Shape<BN>::kStages * Shape<BN>::kStageBytes + sizeof(GroupedShared);
-}
-static_assert(grouped_smem<256>() <= 232448 && grouped_smem<64>() <= 232448,
-              "shared memory of one CTA");
-static_assert(Shape<256>::kStages <= kMaxStages && Shape<64>::kStages <= kMaxStages, "barriers");
+constexpr size_t kGroupedSmem = 1024 + kStages * kStageBytes + sizeof(GroupedShared);
+static_assert(kGroupedSmem <= 232448, "shared memory of one CTA");
 
-template <int BN>
 int launch_grouped(GroupedArgs& A, Operand a, Operand b, int64_t tiles, char* ws,
                    cudaStream_t s) {
     // the runtime calls first: they bind the device's context to a thread that has
@@ -672,18 +660,18 @@ int launch_grouped(GroupedArgs& A, Operand a, Operand b, int64_t tiles, char* ws
     SK_CUDA(cudaGetDevice(&dev));
     SK_CUDA(cudaSetDevice(dev));
     SK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    SK_CUDA(cudaFuncSetAttribute(k_grouped<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)grouped_smem<BN>()));
+    SK_CUDA(cudaFuncSetAttribute(k_grouped, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)kGroupedSmem));
     int rc = a.pack(ws, s);
     if (rc == SK_OK) rc = b.pack(ws, s);
     if (rc == SK_OK) rc = encode(&A.a, a, A.bf16, A.a_mn ? kBK : kBM);
-    if (rc == SK_OK) rc = encode(&A.b, b, A.bf16, A.b_mn ? kBK : Shape<BN>::kHalf);
+    if (rc == SK_OK) rc = encode(&A.b, b, A.bf16, A.b_mn ? kBK : kHalf);
     if (rc == SK_OK) rc = encode(&A.b32, b, A.bf16, A.b_mn ? kBK : 32);
     if (rc != SK_OK) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, sms / 2));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = grouped_smem<BN>();
+    cfg.dynamicSmemBytes = kGroupedSmem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -692,7 +680,7 @@ int launch_grouped(GroupedArgs& A, Operand a, Operand b, int64_t tiles, char* ws
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    SK_CUDA(cudaLaunchKernelEx(&cfg, k_grouped<BN>, A));
+    SK_CUDA(cudaLaunchKernelEx(&cfg, k_grouped, A));
     return SK_OK;
 }
 
@@ -704,13 +692,15 @@ int check_grouped(int dtype, int64_t S, int64_t K, int64_t N, int64_t E, const i
     if (E > kMaxGroups) return fail(SK_ERR_ARG, "at most 1024 groups");
     if (S > (1 << 30) || K > (1 << 30) || N > (1 << 30))
         return fail(SK_ERR_ARG, "S, K and N must be at most 2^30");
+    if (E * std::max(K, N) > INT32_MAX)
+        return fail(SK_ERR_ARG, "E * K and E * N must be below 2^31");
     if (!offsets) return fail(SK_ERR_ARG, "offsets is NULL");
     return SK_OK;
 }
 
 // Tiles of a launch, at most (the runs are known to the device alone).
-int64_t most_tiles(int64_t m, int64_t c, int64_t groups, int bn) {
-    return (m + kPairM - 1) / kPairM * ((c + bn - 1) / bn + groups);
+int64_t most_tiles(int64_t m, int64_t c, int64_t groups) {
+    return (m + kPairM - 1) / kPairM * ((c + kBN - 1) / kBN + groups);
 }
 
 // W_e's axes as an operand: rows of the unit-stride axis.
@@ -720,12 +710,17 @@ Operand weight_operand(const void* w, int64_t E, int64_t K, int64_t N, int64_t s
     return Operand{w, E, N, K, se, sn};
 }
 
-int check_weight(int64_t K, int64_t N, int64_t se, int64_t sk_, int64_t sn) {
+int check_weight(int64_t se, int64_t sk_, int64_t sn) {
     if (se < 0 || sk_ < 0 || sn < 0) return fail(SK_ERR_LAYOUT, "negative strides");
     if (sn != 1 && sk_ != 1)
         return fail(SK_ERR_LAYOUT, "one axis of the weights must have unit stride");
-    (void)K;
-    (void)N;
+    return SK_OK;
+}
+
+int check_workspace(const void* ws, size_t bytes, size_t need, const char* what) {
+    if (need > 0 && (!ws || bytes < need || (uintptr_t)ws % 16 != 0))
+        return fail(SK_ERR_WORKSPACE,
+                    std::string("workspace too small or not 16-byte aligned for ") + what);
     return SK_OK;
 }
 
@@ -750,14 +745,14 @@ int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ld
     using namespace sk;
     clear_error();
     int rc = check_grouped(dtype, S, K, N, E, offsets);
-    if (rc == SK_OK) rc = check_weight(K, N, swe, swk, swn);
+    if (rc == SK_OK) rc = check_weight(swe, swk, swn);
     if (rc != SK_OK) return rc;
     if (!x || !w || !y) return fail(SK_ERR_ARG, "x, w or y is NULL");
     if (ldx < 0) return fail(SK_ERR_LAYOUT, "negative strides");
     const size_t need =
         sk_grouped_matmul_workspace_bytes(x, S, K, ldx, w, E, N, swe, swk, swn);
-    if (need > 0 && (!workspace || workspace_bytes < need))
-        return fail(SK_ERR_WORKSPACE, "workspace too small for sk_grouped_matmul");
+    rc = check_workspace(workspace, workspace_bytes, need, "sk_grouped_matmul");
+    if (rc != SK_OK) return rc;
     GroupedArgs A{};
     A.out = y;
     A.ldo = N;
@@ -770,15 +765,11 @@ int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ld
     A.a_mn = swn == 1;
     A.b_mn = false;
     A.bf16 = dtype == SK_BF16;
-    const int64_t tiles = most_tiles(N, S, E + 2, 64);
+    const int64_t tiles = most_tiles(N, S, E + 2);
     if (tiles > INT32_MAX) return fail(SK_ERR_ARG, "the output has too many tiles");
     const Operand ow = weight_operand(w, E, K, N, swe, swk, swn);
     const Operand ox{x, 1, S, K, 0, ldx};
-    // short groups (32 rows on average): narrow tiles, more weights in flight
-    return S <= 32 * E ? launch_grouped<64>(A, ow, ox, tiles, (char*)workspace,
-                                            (cudaStream_t)stream)
-                       : launch_grouped<256>(A, ow, ox, tiles, (char*)workspace,
-                                             (cudaStream_t)stream);
+    return launch_grouped(A, ow, ox, tiles, (char*)workspace, (cudaStream_t)stream);
 }
 
 size_t sk_grouped_matmul_weight_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
@@ -795,13 +786,13 @@ int sk_grouped_matmul_weight(const void* x, int dtype, int64_t S, int64_t K, int
                              size_t workspace_bytes, void* stream) {
     using namespace sk;
     clear_error();
-    const int rc = check_grouped(dtype, S, K, N, E, offsets);
+    int rc = check_grouped(dtype, S, K, N, E, offsets);
     if (rc != SK_OK) return rc;
     if (!x || !dy || !dw) return fail(SK_ERR_ARG, "x, dy or dw is NULL");
     if (ldx < 0 || ldy < 0) return fail(SK_ERR_LAYOUT, "negative strides");
     const size_t need = sk_grouped_matmul_weight_workspace_bytes(x, S, K, ldx, dy, N, ldy);
-    if (need > 0 && (!workspace || workspace_bytes < need))
-        return fail(SK_ERR_WORKSPACE, "workspace too small for sk_grouped_matmul_weight");
+    rc = check_workspace(workspace, workspace_bytes, need, "sk_grouped_matmul_weight");
+    if (rc != SK_OK) return rc;
     GroupedArgs A{};
     A.out = dw;
     A.out_group = K * N;
@@ -815,10 +806,10 @@ int sk_grouped_matmul_weight(const void* x, int dtype, int64_t S, int64_t K, int
     A.m = (int)(transposed ? K : N);
     A.c = (int)(transposed ? N : K);
     A.ldo = A.m;
-    const int64_t tiles = (A.m + kPairM - 1) / kPairM * (int64_t)((A.c + 255) / 256) * E;
+    const int64_t tiles = (A.m + kPairM - 1) / kPairM * (int64_t)((A.c + kBN - 1) / kBN) * E;
     if (tiles > INT32_MAX) return fail(SK_ERR_ARG, "the output has too many tiles");
-    return launch_grouped<256>(A, transposed ? ox : og, transposed ? og : ox, tiles,
-                               (char*)workspace, (cudaStream_t)stream);
+    return launch_grouped(A, transposed ? ox : og, transposed ? og : ox, tiles,
+                          (char*)workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

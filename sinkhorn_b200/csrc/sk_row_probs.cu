@@ -1587,7 +1587,8 @@ int sk_row_logprobs(const void* X, int dtype, int64_t B, int64_t N, int64_t M, i
     if (top_k > 0 && (!top_logprob || !top_index))
         return fail(SK_ERR_ARG, "top_k needs top_logprob and top_index");
     if (mask_b && M > kStagedMax &&
-        (!workspace || workspace_bytes < sk_row_logprobs_workspace_bytes(B, M)))
+        (!workspace || (uintptr_t)workspace % 16 != 0 ||
+         workspace_bytes < sk_row_logprobs_workspace_bytes(B, M)))
         return fail(SK_ERR_WORKSPACE, "workspace too small for sk_row_logprobs with mask_b");
     cudaStream_t s = (cudaStream_t)stream;
     RowProbArgs A{};
@@ -1652,8 +1653,9 @@ int sk_row_logprobs_backward(const void* X, int dtype, int64_t B, int64_t N, int
         return fail(SK_ERR_ARG, "grad_top needs top_k and top_index");
     if (!dX && !dg) return fail(SK_ERR_ARG, "dX and dg are both NULL");
     if (dX && (uintptr_t)dX % 16 != 0) return fail(SK_ERR_LAYOUT, "dX is not 16-byte aligned");
-    if ((dg || mask_b) && (!workspace || workspace_bytes <
-                                             sk_row_logprobs_backward_workspace_bytes(B, N, M)))
+    if ((dg || mask_b) &&
+        (!workspace || (uintptr_t)workspace % 16 != 0 ||
+         workspace_bytes < sk_row_logprobs_backward_workspace_bytes(B, N, M)))
         return fail(SK_ERR_WORKSPACE, "workspace too small for sk_row_logprobs_backward");
     cudaStream_t s = (cudaStream_t)stream;
     const int fm = fold_mask(&g, mask_b, B * M, workspace, s);

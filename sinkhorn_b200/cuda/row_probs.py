@@ -32,8 +32,8 @@ def row_probs(X: Tensor, g: Tensor | None, epsilon: float, negate: bool,
     if B * N:
         lib = T.lib()
         with T.on(dev):
-            ws = None if mask_b is None else T.workspace(
-                lib.sk_row_logprobs_workspace_bytes(B, M), dev)
+            need = 0 if mask_b is None else lib.sk_row_logprobs_workspace_bytes(B, M)
+            ws = T.workspace(need, dev) if need else None
             rc = lib.sk_row_logprobs(
                 X.data_ptr(), T.DTYPES[X.dtype], B, N, M, *X.stride(), T.ptr(g), epsilon,
                 int(negate), T.ptr(mask_a), T.ptr(mask_b), T.ptr(targets), top_k,
