@@ -586,6 +586,7 @@ int sk_row_logprobs_backward(const void* X, int dtype, int64_t B, int64_t N, int
 /* ---------------------------------------------------------------------- */
 /* Experts: rows into the order of their experts and back.                 */
 
+/* Workspace bytes of sk_expert_dispatch (0 up to 2048 slots). */
 size_t sk_expert_dispatch_workspace_bytes(int64_t slots, int experts);
 
 /*
@@ -628,36 +629,34 @@ int sk_combine_rows_backward(const void* grad_out, const void* y, int dtype, int
                              const int* offsets, int experts, const float* weights, void* grad_y,
                              float* grad_weights, void* stream);
 
-/* Workspace bytes of sk_grouped_matmul: 0 when x and w start every row on 16
- * bytes (only the addresses' alignment is looked at). */
-size_t sk_grouped_matmul_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
-                                         const void* w, int64_t E, int64_t N, int64_t swe,
-                                         int64_t swk, int64_t swn);
+/*
+ * dst[g][r][0..ld) = src[g * sg + r * sr + 0..width) of 16-bit elements, ld =
+ * width rounded up to 8, the padding 0: an operand of the products below whose
+ * rows do not start on 16 bytes, laid out so that they do.
+ */
+int sk_grouped_pack(const void* src, int64_t groups, int64_t rows, int64_t width, int64_t sg,
+                    int64_t sr, void* dst, void* stream);
 
 /*
  * y[r] = x[r] W_e for the rows r of group e, offsets[e] <= r < offsets[e+1];
  * rows of no group are zero. x (S,K) with row stride ldx, W (E,K,N) with
  * element strides swe, swk, swn (swk or swn is 1), y (S,N) dense; all bf16 or
- * all fp16, sums in fp32, rounded once. offsets (E+1) is device memory;
- * entries that fall or leave [0,S] are brought back. E <= 1024. The gradient
- * of x is the same call on dy with K, N and swk, swn exchanged.
+ * all fp16, sums in fp32, rounded once. Every row of x and W starts on 16 bytes
+ * (address and strides; else SK_ERR_LAYOUT: sk_grouped_pack). offsets (E+1) is
+ * device memory; entries that fall or leave [0,S] are brought back. E <= 1024.
+ * The gradient of x is the same call on dy with K, N and swk, swn exchanged.
  */
 int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ldx, const void* w,
                       int64_t E, int64_t N, int64_t swe, int64_t swk, int64_t swn,
-                      const int* offsets, void* y, void* workspace, size_t workspace_bytes,
-                      void* stream);
-
-size_t sk_grouped_matmul_weight_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
-                                                const void* dy, int64_t N, int64_t ldy);
+                      const int* offsets, void* y, void* stream);
 
 /*
  * dW_e = sum over the rows r of group e of x[r]^T dy[r]: (E,K,N) dense, or
- * (E,N,K) dense when `transposed`; zero for a group without rows.
+ * (E,N,K) dense when `transposed`; zero for a group without rows. Rows as above.
  */
 int sk_grouped_matmul_weight(const void* x, int dtype, int64_t S, int64_t K, int64_t ldx,
                              const void* dy, int64_t N, int64_t ldy, const int* offsets,
-                             int64_t E, void* dw, int transposed, void* workspace,
-                             size_t workspace_bytes, void* stream);
+                             int64_t E, void* dw, int transposed, void* stream);
 
 #ifdef __cplusplus
 }

@@ -118,13 +118,11 @@ SIGNATURES = {
     "sk_combine_rows": (_INT, [_P, _INT, _I64, _INT, _I64, _I64, _P, _P, _INT, _P, _P, _P]),
     "sk_combine_rows_backward": (_INT, [_P, _P, _INT, _I64, _INT, _I64, _I64, _I64, _P, _P,
                                         _INT, _P, _P, _P, _P]),
-    "sk_grouped_matmul_workspace_bytes": (_SZ, [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64,
-                                                _I64, _I64]),
+    "sk_grouped_pack": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P]),
     "sk_grouped_matmul": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,
-                                 _P, _P, _P, _SZ, _P]),
-    "sk_grouped_matmul_weight_workspace_bytes": (_SZ, [_P, _I64, _I64, _I64, _P, _I64, _I64]),
+                                 _P, _P, _P]),
     "sk_grouped_matmul_weight": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64,
-                                        _P, _INT, _P, _SZ, _P]),
+                                        _P, _INT, _P]),
 }
 
 _lock = threading.Lock()

@@ -407,7 +407,7 @@ int64_t sort_tiles(int64_t S) { return (S + kSortTile - 1) / kSortTile; }
 extern "C" {
 
 size_t sk_expert_dispatch_workspace_bytes(int64_t slots, int experts) {
-    if (slots <= 0 || experts <= 0) return 0;
+    if (slots <= sk::kSortTile || experts <= 0) return 0;  // one CTA counts for itself
     return sk::align_up(sizeof(int) * (size_t)sk::sort_tiles(slots) * experts);
 }
 
@@ -421,7 +421,8 @@ int sk_expert_dispatch(const int64_t* index, int64_t slots, int experts, int* or
     if (slots <= 0 || slots > INT32_MAX) return fail(SK_ERR_ARG, "slots must lie in 1..2^31-1");
     if (experts <= 0 || experts > kMaxExperts)
         return fail(SK_ERR_ARG, "experts must lie in 1..1024");
-    if (!workspace || workspace_bytes < sk_expert_dispatch_workspace_bytes(slots, experts))
+    const size_t need = sk_expert_dispatch_workspace_bytes(slots, experts);
+    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4 != 0))
         return fail(SK_ERR_WORKSPACE, "workspace too small for sk_expert_dispatch");
     cudaStream_t s = (cudaStream_t)stream;
     const int tiles = (int)sort_tiles(slots);

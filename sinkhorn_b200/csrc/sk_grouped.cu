@@ -216,16 +216,23 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
 // The accumulators to memory. D has the output's contiguous dimension on the
 // lanes, so 32 x 32 pieces are turned in the warp's corner of shared memory: 16-bit
 // fragments are stored transposed, and leave as 16-byte pieces of output rows, 8
-// rows of 64 bytes to an instruction. Outputs whose rows do not start on 16
-// bytes leave element by element.
+// rows of 64 bytes to an instruction. Where output rows do not start on 16 bytes a
+// lane stores its elements one by one: 64 consecutive bytes of a row to an
+// instruction (pairs read back from the corner were slower, 56 us against 20 us
+// for 5003 x 1001 x 777).
+// Byte of lane m of column `row` in the corner: 32 rows of 64 bytes, whose four
+// 16-byte pieces are turned by the row's bits 1 and 2, which spreads the accesses
+// over all banks.
+__device__ __forceinline__ int turned(int row, int m) {
+    return row * 64 + ((m >> 3 ^ (row >> 1 & 3)) << 4) + (m & 7) * 2;
+}
+
 template <typename T>
 __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh, int rank,
                                          int quarter, int lane) {
     int used = 0;  // accumulators so far
     const uint32_t release0 = map_to_rank(&sh->acc_empty[0], 0);
     const uint32_t release1 = map_to_rank(&sh->acc_empty[1], 0);
-    // 32 rows (columns of D) of 64 bytes, the four 16-byte pieces of a row turned
-    // by the row's bits 1 and 2, which spreads both accesses over all banks
     uint8_t* const turn = sh->turn[quarter];
     const uint32_t turn0 = smem_u32(turn);
     const bool wide = A.ldo % 8 == 0 && A.m % 8 == 0 && A.out_group % 8 == 0 &&
@@ -246,10 +253,9 @@ __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh
         const uint32_t acc = sh->tmem + ((uint32_t)(quarter * 32) << 16) + buf * kBN;
         const uint32_t fill = __float_as_uint(ok ? 0.f : NAN);
         if (wide) {
-            // piece p = lane % 4 of rows lane / 4 + 8 i
-            const int piece = lane & 3, r0 = lane >> 2;
-            const bool in = m0 + piece * 8 < A.m;
-            T* o = out + (int64_t)r0 * A.ldo + piece * 8;
+            // piece lane % 4 of rows lane / 4 + 8 i
+            const int r0 = lane >> 2, m = (lane & 3) * 8;
+            T* o = out + (int64_t)r0 * A.ldo + m;
             for (int c = 0; c < q.cols; c += 32) {
                 uint32_t v[2][16];
                 if (held) {
@@ -279,22 +285,21 @@ __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh
                         // matrix l / 8: its lanes 16 h + 8 (l / 8 % 2), columns 16 g + 8 (l / 16)
                         const int row = 16 * g + 8 * (lane >> 4) + (lane & 7);
                         const int p = 2 * h + (lane >> 3 & 1);
-                        st_matrix4_trans(turn0 + row * 64 + ((p ^ (row >> 1 & 3)) << 4), w[0],
-                                         w[1], w[2], w[3]);
+                        st_matrix4_trans(turn0 + turned(row, p * 8), w[0], w[1], w[2], w[3]);
                     }
                 }
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = r0 + 8 * i;
-                    const uint4 x = *reinterpret_cast<const uint4*>(
-                        turn + row * 64 + ((piece ^ (row >> 1 & 3)) << 4));
-                    if (in && c + row < q.cols)
+                    const uint4 x = *reinterpret_cast<const uint4*>(turn + turned(row, m));
+                    if (m0 + m < A.m && c + row < q.cols)
                         *reinterpret_cast<uint4*>(o + (int64_t)i * 8 * A.ldo) = x;
                 }
                 o += 32 * A.ldo;
             }
         } else {
+            T* o = out + lane;
             for (int c = 0; c < q.cols; c += 32) {
                 uint32_t v[32];
                 if (held) {
@@ -304,10 +309,17 @@ __device__ __forceinline__ void epilogue(const GroupedArgs& A, GroupedShared* sh
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = fill;
                 }
+                if (m0 + lane < A.m) {
+                    if (c + 32 <= q.cols) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (c + i < q.cols && m0 + lane < A.m)
-                        out[(int64_t)(c + i) * A.ldo + lane] = (T)__uint_as_float(v[i]);
+                        for (int i = 0; i < 32; ++i, o += A.ldo) *o = (T)__uint_as_float(v[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i, o += A.ldo)
+                            if (c + i < q.cols) *o = (T)__uint_as_float(v[i]);
+                    }
+                }
+                __syncwarp();
             }
             if (q.depth > 0) {
                 tc_fence_before();
@@ -587,26 +599,10 @@ struct Operand {
     const void* p;
     int64_t groups, rows, width, sg, sr;
 
-    bool ready() const {
+    // what the copy engine takes: every row starts on 16 bytes
+    bool aligned() const {
         return (uintptr_t)p % 16 == 0 && (rows == 1 || (sr % 8 == 0 && sr >= 8)) &&
                (groups == 1 || (sg % 8 == 0 && sg >= 8));
-    }
-    size_t packed_bytes() const {
-        return ready() ? 0 : align_up((size_t)groups * rows * ((width + 7) / 8 * 8) * 2);
-    }
-    int pack(char*& ws, cudaStream_t s) {
-        if (ready()) return SK_OK;
-        const int64_t ld = (width + 7) / 8 * 8, total = groups * rows * (ld / 8);
-        const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 32);
-        k_grouped_pack<<<grid, 256, 0, s>>>((const uint16_t*)p, sg, sr, (unsigned)rows,
-                                            (int)width, (unsigned)(ld / 8), total, (uint4*)ws);
-        SK_LAUNCHED("k_grouped_pack");
-        const size_t used = packed_bytes();
-        p = ws;
-        sr = ld;
-        sg = ld * rows;
-        ws += used;
-        return SK_OK;
     }
 };
 
@@ -652,8 +648,10 @@ int encode(CUtensorMap* map, const Operand& o, bool bf16, uint32_t box_rows) {
 constexpr size_t kGroupedSmem = 1024 + kStages * kStageBytes + sizeof(GroupedShared);
 static_assert(kGroupedSmem <= 232448, "shared memory of one CTA");
 
-int launch_grouped(GroupedArgs& A, Operand a, Operand b, int64_t tiles, char* ws,
+int launch_grouped(GroupedArgs& A, const Operand& a, const Operand& b, int64_t tiles,
                    cudaStream_t s) {
+    if (!a.aligned() || !b.aligned())
+        return fail(SK_ERR_LAYOUT, "operand rows must start on 16 bytes (sk_grouped_pack)");
     // the runtime calls first: they bind the device's context to a thread that has
     // none yet (autograd's), which the map encoder needs
     int dev = 0, sms = 0;
@@ -662,9 +660,7 @@ int launch_grouped(GroupedArgs& A, Operand a, Operand b, int64_t tiles, char* ws
     SK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     SK_CUDA(cudaFuncSetAttribute(k_grouped, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)kGroupedSmem));
-    int rc = a.pack(ws, s);
-    if (rc == SK_OK) rc = b.pack(ws, s);
-    if (rc == SK_OK) rc = encode(&A.a, a, A.bf16, A.a_mn ? kBK : kBM);
+    int rc = encode(&A.a, a, A.bf16, A.a_mn ? kBK : kBM);
     if (rc == SK_OK) rc = encode(&A.b, b, A.bf16, A.b_mn ? kBK : kHalf);
     if (rc == SK_OK) rc = encode(&A.b32, b, A.bf16, A.b_mn ? kBK : 32);
     if (rc != SK_OK) return rc;
@@ -717,31 +713,35 @@ int check_weight(int64_t se, int64_t sk_, int64_t sn) {
     return SK_OK;
 }
 
-int check_workspace(const void* ws, size_t bytes, size_t need, const char* what) {
-    if (need > 0 && (!ws || bytes < need || (uintptr_t)ws % 16 != 0))
-        return fail(SK_ERR_WORKSPACE,
-                    std::string("workspace too small or not 16-byte aligned for ") + what);
-    return SK_OK;
-}
-
 }  // namespace
 }  // namespace sk
 
 extern "C" {
 
-size_t sk_grouped_matmul_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
-                                         const void* w, int64_t E, int64_t N, int64_t swe,
-                                         int64_t swk, int64_t swn) {
+int sk_grouped_pack(const void* src, int64_t groups, int64_t rows, int64_t width, int64_t sg,
+                    int64_t sr, void* dst, void* stream) {
     using namespace sk;
-    if (S <= 0 || K <= 0 || N <= 0 || E <= 0) return 0;
-    return Operand{x, 1, S, K, 0, ldx}.packed_bytes() +
-           weight_operand(w, E, K, N, swe, swk, swn).packed_bytes();
+    clear_error();
+    if (!src || !dst) return fail(SK_ERR_ARG, "src or dst is NULL");
+    if (groups <= 0 || rows <= 0 || width <= 0)
+        return fail(SK_ERR_ARG, "groups, rows and width must be positive");
+    if (rows > INT32_MAX || width > (1 << 30) || groups > INT32_MAX / rows)
+        return fail(SK_ERR_ARG, "groups * rows must be below 2^31 and width at most 2^30");
+    if (sg < 0 || sr < 0) return fail(SK_ERR_LAYOUT, "negative strides");
+    if ((uintptr_t)src % 2 != 0 || (uintptr_t)dst % 16 != 0)
+        return fail(SK_ERR_LAYOUT, "src must be 2-byte and dst 16-byte aligned");
+    const int64_t pieces = (width + 7) / 8, total = groups * rows * pieces;
+    const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 32);
+    k_grouped_pack<<<grid, 256, 0, (cudaStream_t)stream>>>((const uint16_t*)src, sg, sr,
+                                                           (unsigned)rows, (int)width,
+                                                           (unsigned)pieces, total, (uint4*)dst);
+    SK_LAUNCHED("k_grouped_pack");
+    return SK_OK;
 }
 
 int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ldx, const void* w,
                       int64_t E, int64_t N, int64_t swe, int64_t swk, int64_t swn,
-                      const int* offsets, void* y, void* workspace, size_t workspace_bytes,
-                      void* stream) {
+                      const int* offsets, void* y, void* stream) {
     using namespace sk;
     clear_error();
     int rc = check_grouped(dtype, S, K, N, E, offsets);
@@ -749,10 +749,6 @@ int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ld
     if (rc != SK_OK) return rc;
     if (!x || !w || !y) return fail(SK_ERR_ARG, "x, w or y is NULL");
     if (ldx < 0) return fail(SK_ERR_LAYOUT, "negative strides");
-    const size_t need =
-        sk_grouped_matmul_workspace_bytes(x, S, K, ldx, w, E, N, swe, swk, swn);
-    rc = check_workspace(workspace, workspace_bytes, need, "sk_grouped_matmul");
-    if (rc != SK_OK) return rc;
     GroupedArgs A{};
     A.out = y;
     A.ldo = N;
@@ -769,30 +765,18 @@ int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ld
     if (tiles > INT32_MAX) return fail(SK_ERR_ARG, "the output has too many tiles");
     const Operand ow = weight_operand(w, E, K, N, swe, swk, swn);
     const Operand ox{x, 1, S, K, 0, ldx};
-    return launch_grouped(A, ow, ox, tiles, (char*)workspace, (cudaStream_t)stream);
-}
-
-size_t sk_grouped_matmul_weight_workspace_bytes(const void* x, int64_t S, int64_t K, int64_t ldx,
-                                                const void* dy, int64_t N, int64_t ldy) {
-    using namespace sk;
-    if (S <= 0 || K <= 0 || N <= 0) return 0;
-    return Operand{x, 1, S, K, 0, ldx}.packed_bytes() +
-           Operand{dy, 1, S, N, 0, ldy}.packed_bytes();
+    return launch_grouped(A, ow, ox, tiles, (cudaStream_t)stream);
 }
 
 int sk_grouped_matmul_weight(const void* x, int dtype, int64_t S, int64_t K, int64_t ldx,
                              const void* dy, int64_t N, int64_t ldy, const int* offsets,
-                             int64_t E, void* dw, int transposed, void* workspace,
-                             size_t workspace_bytes, void* stream) {
+                             int64_t E, void* dw, int transposed, void* stream) {
     using namespace sk;
     clear_error();
-    int rc = check_grouped(dtype, S, K, N, E, offsets);
+    const int rc = check_grouped(dtype, S, K, N, E, offsets);
     if (rc != SK_OK) return rc;
     if (!x || !dy || !dw) return fail(SK_ERR_ARG, "x, dy or dw is NULL");
     if (ldx < 0 || ldy < 0) return fail(SK_ERR_LAYOUT, "negative strides");
-    const size_t need = sk_grouped_matmul_weight_workspace_bytes(x, S, K, ldx, dy, N, ldy);
-    rc = check_workspace(workspace, workspace_bytes, need, "sk_grouped_matmul_weight");
-    if (rc != SK_OK) return rc;
     GroupedArgs A{};
     A.out = dw;
     A.out_group = K * N;
@@ -809,7 +793,7 @@ int sk_grouped_matmul_weight(const void* x, int dtype, int64_t S, int64_t K, int
     const int64_t tiles = (A.m + kPairM - 1) / kPairM * (int64_t)((A.c + kBN - 1) / kBN) * E;
     if (tiles > INT32_MAX) return fail(SK_ERR_ARG, "the output has too many tiles");
     return launch_grouped(A, transposed ? ox : og, transposed ? og : ox, tiles,
-                          (char*)workspace, (cudaStream_t)stream);
+                          (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -14,17 +14,18 @@ from .. import _tensors as T
 def sort_slots(index: Tensor, n_experts: int) -> tuple[Tensor, Tensor, Tensor]:
     """sk_expert_dispatch on a dense int64 index (T, k): (order, position, offsets)."""
     dev, slots = index.device, index.numel()
-    order = torch.empty(slots, device=dev, dtype=torch.int32)
     position = torch.empty(index.shape, device=dev, dtype=torch.int32)
+    order = position.new_empty(slots)
     if not slots:
         return order, position, torch.zeros(n_experts + 1, device=dev, dtype=torch.int32)
-    offsets = torch.empty(n_experts + 1, device=dev, dtype=torch.int32)
+    offsets = position.new_empty(n_experts + 1)
     lib = T.lib()
     with T.on(dev):
-        ws = T.workspace(lib.sk_expert_dispatch_workspace_bytes(slots, n_experts), dev)
+        need = lib.sk_expert_dispatch_workspace_bytes(slots, n_experts)
+        ws = T.workspace(need, dev) if need else None
         rc = lib.sk_expert_dispatch(index.data_ptr(), slots, n_experts, order.data_ptr(),
-                                    position.data_ptr(), offsets.data_ptr(), ws.data_ptr(),
-                                    ws.numel(), T.stream_of(dev))
+                                    position.data_ptr(), offsets.data_ptr(), T.ptr(ws), need,
+                                    T.stream_of(dev))
         T.check(rc, "sk_expert_dispatch")
     return order, position, offsets
 
@@ -91,20 +92,53 @@ def sum_rows_backward(grad: Tensor, y: Tensor, position: Tensor, offsets: Tensor
     return dy, dw
 
 
-def _weight_strides(w: Tensor) -> tuple[int, int, int]:
-    """Strides of w (E, K, N); an axis of one element has stride 1."""
-    return tuple(s if n > 1 else 1 for s, n in zip(w.stride(), w.shape))
+def _strides(t: Tensor) -> tuple:
+    """Strides of t; an axis of one element has stride 1."""
+    return tuple(s if n > 1 else 1 for s, n in zip(t.stride(), t.shape))
 
 
-def unit_weights(w: Tensor) -> Tensor:
-    """w itself where one of its last two axes has unit stride, else a dense copy."""
-    _, sk, sn = _weight_strides(w)
-    return w if sk == 1 or sn == 1 else w.contiguous()
+def _on_grid(t: Tensor, *strides: int) -> bool:
+    return t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 8 for s in strides)
+
+
+def _packed(t: Tensor, sg: int, sr: int) -> Tensor:
+    """sk_grouped_pack: t (groups, rows, width), unit column stride, with rows on 16
+    bytes; a view of its width."""
+    groups, rows, width = t.shape
+    dst = torch.empty(groups, rows, (width + 7) // 8 * 8, device=t.device, dtype=t.dtype)
+    with T.on(t.device):
+        rc = T.lib().sk_grouped_pack(t.data_ptr(), groups, rows, width, sg, sr,
+                                     dst.data_ptr(), T.stream_of(t.device))
+        T.check(rc, "sk_grouped_pack")
+    return dst[:, :, :width]
+
+
+def aligned_rows(x: Tensor) -> Tensor:
+    """x (S, K) with unit column stride and every row on 16 bytes: itself or a copy."""
+    x = unit_rows(x)
+    if not x.numel() or _on_grid(x, *([x.stride(0)] if x.shape[0] > 1 else [])):
+        return x
+    return _packed(x.unsqueeze(0), 0, x.stride(0))[0]
+
+
+def aligned_weights(w: Tensor) -> Tensor:
+    """w (E, K, N) with one of its last two axes of unit stride and every row of that
+    axis on 16 bytes: itself or a copy."""
+    se, sk, sn = _strides(w)
+    if sk != 1 and sn != 1:
+        w = w.contiguous()
+        se, sk, sn = _strides(w)
+    if sn != 1 or (w.shape[2] == 1 and w.shape[1] > 1 and sk == 1):
+        return aligned_weights(w.transpose(1, 2)).transpose(1, 2)
+    rows = ([sk] if w.shape[1] > 1 else []) + ([se] if w.shape[0] > 1 else [])
+    if not w.numel() or _on_grid(w, *rows):
+        return w
+    return _packed(w, se, sk)
 
 
 def product(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
-    """sk_grouped_matmul: (S, N) from x (S, K), w (E, K, N) (unit_weights) and offsets."""
-    x = unit_rows(x)
+    """sk_grouped_matmul: (S, N) from x (S, K) (aligned_rows), w (E, K, N)
+    (aligned_weights, or transposed) and offsets."""
     S, K = x.shape
     E, _, N = w.shape
     y = torch.empty(S, N, device=x.device, dtype=x.dtype)
@@ -112,34 +146,27 @@ def product(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
         return y
     if not K:
         return y.zero_()
-    lib = T.lib()
     with T.on(x.device):
-        args = (S, K, x.stride(0), w.data_ptr(), E, N, *_weight_strides(w))
-        n = lib.sk_grouped_matmul_workspace_bytes(x.data_ptr(), *args)
-        ws = T.workspace(n, x.device) if n else None
-        rc = lib.sk_grouped_matmul(x.data_ptr(), T.DTYPES[x.dtype], *args, offsets.data_ptr(),
-                                   y.data_ptr(), T.ptr(ws), n, T.stream_of(x.device))
+        rc = T.lib().sk_grouped_matmul(
+            x.data_ptr(), T.DTYPES[x.dtype], S, K, x.stride(0), w.data_ptr(), E, N,
+            *_strides(w), offsets.data_ptr(), y.data_ptr(), T.stream_of(x.device))
         T.check(rc, "sk_grouped_matmul")
     return y
 
 
 def weight_product(x: Tensor, dy: Tensor, offsets: Tensor, transposed: bool) -> Tensor:
-    """sk_grouped_matmul_weight: dW (E, K, N), laid out (E, N, K) when ``transposed``."""
-    x, dy = unit_rows(x), unit_rows(dy)
+    """sk_grouped_matmul_weight on aligned_rows: dW (E, K, N), laid out (E, N, K) when
+    ``transposed``."""
     S, K = x.shape
     N, E = dy.shape[1], offsets.numel() - 1
     dw = torch.empty((E, N, K) if transposed else (E, K, N), device=x.device, dtype=x.dtype)
     if not S:
         dw.zero_()
     elif dw.numel():
-        lib = T.lib()
         with T.on(x.device):
-            n = lib.sk_grouped_matmul_weight_workspace_bytes(
-                x.data_ptr(), S, K, x.stride(0), dy.data_ptr(), N, dy.stride(0))
-            ws = T.workspace(n, x.device) if n else None
-            rc = lib.sk_grouped_matmul_weight(
+            rc = T.lib().sk_grouped_matmul_weight(
                 x.data_ptr(), T.DTYPES[x.dtype], S, K, x.stride(0), dy.data_ptr(), N,
                 dy.stride(0), offsets.data_ptr(), E, dw.data_ptr(), int(transposed),
-                T.ptr(ws), n, T.stream_of(x.device))
+                T.stream_of(x.device))
             T.check(rc, "sk_grouped_matmul_weight")
     return dw.transpose(1, 2) if transposed else dw

@@ -22,9 +22,9 @@ def row_probs(X: Tensor, g: Tensor | None, epsilon: float, negate: bool,
     dev = X.device
     f32 = torch.float32
     lse = torch.empty(lead, device=dev, dtype=f32)
-    entropy = torch.empty(lead, device=dev, dtype=f32)
+    entropy = torch.empty_like(lse)
     stats = torch.empty((B, N, 2), device=dev, dtype=f32) if keep else None
-    logprob = torch.empty(lead, device=dev, dtype=f32) if targets is not None else None
+    logprob = torch.empty_like(lse) if targets is not None else None
     top_lp = top_idx = None
     if top_k:
         top_lp = torch.empty((*lead, top_k), device=dev, dtype=f32)

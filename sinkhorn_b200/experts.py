@@ -18,8 +18,8 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _tensors as T
-from .cuda.experts import (gather_rows, product, sort_slots, sum_rows, sum_rows_backward,
-                           unit_weights, weight_product)
+from .cuda.experts import (aligned_rows, aligned_weights, gather_rows, product, sort_slots,
+                           sum_rows, sum_rows_backward, weight_product)
 
 MAX_EXPERTS = 1024
 
@@ -159,7 +159,9 @@ def combine_rows(y: Tensor, dispatch: ExpertDispatch, weights: Tensor | None = N
 class GroupedMatmulFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
+        x, w = aligned_rows(x), aligned_weights(w)
         ctx.save_for_backward(x, w, offsets)
+        ctx.transposed = w.stride(2) != 1 and w.shape[2] > 1
         return product(x, w, offsets)
 
     @staticmethod
@@ -167,10 +169,11 @@ class GroupedMatmulFunction(torch.autograd.Function):
     def backward(ctx: Any, grad: Tensor):
         x, w, offsets = ctx.saved_tensors
         dx = dw = None
+        grad = aligned_rows(grad)
         if ctx.needs_input_grad[0]:
             dx = product(grad, w.transpose(1, 2), offsets)
         if ctx.needs_input_grad[1]:
-            dw = weight_product(x, grad, offsets, transposed=w.stride(2) != 1)
+            dw = weight_product(x, grad, offsets, ctx.transposed)
         return dx, dw, None
 
 
@@ -210,7 +213,6 @@ def grouped_matmul(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
     if offsets.dtype == torch.int64:
         offsets = offsets.clamp(0, x.shape[0]).to(torch.int32)
     offsets = offsets.contiguous()
-    w = unit_weights(w)
     if not T.needs_grad(x, w):
-        return product(x, w, offsets)
+        return product(aligned_rows(x), aligned_weights(w), offsets)
     return GroupedMatmulFunction.apply(x, w, offsets)

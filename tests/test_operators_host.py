@@ -141,14 +141,12 @@ def _rows_bwd(L, X=_P, stats=_P, t=None, k=0, ti=None, ent=None, glp=None, gent=
                                       ent, None, glp, gent, gtop, dX, dg, ws, wsb, None)
 
 
-def _gmm(L, x=_P, dt=1, S=16, K=64, ldx=64, w=_P, E=2, N=32, se=2048, sk=32, sn=1, o=_P, y=_P,
-         ws=None, wsb=0):
-    return L.sk_grouped_matmul(x, dt, S, K, ldx, w, E, N, se, sk, sn, o, y, ws, wsb, None)
+def _gmm(L, x=_P, dt=1, S=16, K=64, ldx=64, w=_P, E=2, N=32, se=2048, sk=32, sn=1, o=_P, y=_P):
+    return L.sk_grouped_matmul(x, dt, S, K, ldx, w, E, N, se, sk, sn, o, y, None)
 
 
-def _gmw(L, x=_P, dt=1, S=16, K=64, ldx=64, dy=_P, N=32, ldy=32, o=_P, E=2, dw=_P, ws=None,
-         wsb=0):
-    return L.sk_grouped_matmul_weight(x, dt, S, K, ldx, dy, N, ldy, o, E, dw, 0, ws, wsb, None)
+def _gmw(L, x=_P, dt=1, S=16, K=64, ldx=64, dy=_P, N=32, ldy=32, o=_P, E=2, dw=_P):
+    return L.sk_grouped_matmul_weight(x, dt, S, K, ldx, dy, N, ldy, o, E, dw, 0, None)
 
 
 _ENTRIES = [
@@ -178,7 +176,8 @@ _ENTRIES = [
     ("sort no slots", lambda L: L.sk_expert_dispatch(_P, 0, 2, _P, _P, _P, _P, _W, None), ARG),
     ("sort 1025 experts", lambda L: L.sk_expert_dispatch(_P, 4, 1025, _P, _P, _P, _P, _W, None),
      ARG),
-    ("sort no workspace", lambda L: L.sk_expert_dispatch(_P, 4, 2, _P, _P, _P, None, 0, None), WS),
+    ("sort no workspace", lambda L: L.sk_expert_dispatch(_P, 2049, 2, _P, _P, _P, None, 0, None),
+     WS),
     ("dispatch x=NULL", lambda L: L.sk_dispatch_rows(None, 1, 4, 2, 8, 8, _P, _P, 2, _P, None),
      ARG),
     ("dispatch T k", lambda L: L.sk_dispatch_rows(_P, 1, 1 << 30, 4, 8, 8, _P, _P, 2, _P, None),
@@ -204,12 +203,18 @@ _ENTRIES = [
     ("product y=NULL", lambda L: _gmm(L, y=None), ARG),
     ("product weights without a unit stride", lambda L: _gmm(L, sk=64, sn=2), LAYOUT),
     ("product negative stride", lambda L: _gmm(L, ldx=-64), LAYOUT),
-    ("product unaligned, no workspace", lambda L: _gmm(L, ldx=65), WS),
-    ("product unaligned, odd workspace", lambda L: _gmm(L, ldx=65, ws=_P + 2, wsb=_W), WS),
+    ("product unaligned stride", lambda L: _gmm(L, ldx=65), LAYOUT),
+    ("product unaligned address", lambda L: _gmm(L, w=_P + 2), LAYOUT),
+    ("product overlapping rows", lambda L: _gmm(L, ldx=0), LAYOUT),
+    ("pack src=NULL", lambda L: L.sk_grouped_pack(None, 1, 4, 7, 28, 7, _P, None), ARG),
+    ("pack no rows", lambda L: L.sk_grouped_pack(_P, 1, 0, 7, 28, 7, _P, None), ARG),
+    ("pack rows", lambda L: L.sk_grouped_pack(_P, 1 << 20, 1 << 20, 7, 28, 7, _P, None), ARG),
+    ("pack stride", lambda L: L.sk_grouped_pack(_P, 1, 4, 7, 28, -7, _P, None), LAYOUT),
+    ("pack dst", lambda L: L.sk_grouped_pack(_P, 1, 4, 7, 28, 7, _P + 8, None), LAYOUT),
     ("product too many tiles", lambda L: _gmm(L, S=1 << 30, K=8, N=1 << 20, sk=1 << 20,
                                               se=1 << 23), ARG),
     ("weight product dw=NULL", lambda L: _gmw(L, dw=None), ARG),
-    ("weight product unaligned", lambda L: _gmw(L, ldy=33), WS),
+    ("weight product unaligned", lambda L: _gmw(L, ldy=33), LAYOUT),
 ]
 
 
@@ -229,14 +234,8 @@ def test_workspace_sizes():
     assert L.sk_row_logprobs_workspace_bytes(4, 16385) >= 4 * 4 * 16385
     assert L.sk_row_logprobs_backward_workspace_bytes(0, 8, 8) == 0
     assert L.sk_row_logprobs_backward_workspace_bytes(2, 100, 64) >= 2 * 4 * 2 * 64
+    assert L.sk_expert_dispatch_workspace_bytes(2048, 8) == 0
     assert L.sk_expert_dispatch_workspace_bytes(5000, 8) >= 3 * 8 * 4
-    # 0 where every row starts on 16 bytes
-    size = L.sk_grouped_matmul_workspace_bytes
-    assert size(_P, 16, 64, 64, _P, 2, 32, 2048, 32, 1) == 0
-    assert size(_P, 16, 63, 63, _P, 2, 32, 2016, 32, 1) >= 16 * 64 * 2
-    assert size(_P + 2, 16, 64, 64, _P, 2, 31, 1984, 31, 1) >= 16 * 64 * 2 + 2 * 64 * 32 * 2
-    assert size(_P, 16, 64, 64, _P, 2, 32, 2048, 1, 64) == 0  # stored (E, N, K)
-    assert L.sk_grouped_matmul_weight_workspace_bytes(_P, 16, 64, 64, _P, 32, 32) == 0
 
 
 def test_public_names():
