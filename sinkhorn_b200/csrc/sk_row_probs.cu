@@ -49,7 +49,6 @@ struct RowProbArgs {
     int64_t B;
     int per_cta;            // rows of one item to a CTA
     unsigned groups;        // CTAs of an item
-    int stages;             // of each warp's ring
     bool staged;            // each CTA holds g (and mask_b) in shared memory
     const float* g;         // (B,M) or NULL; -inf where mask_b leaves a column out
     const uint8_t* mask_b;  // (B,M) or NULL: still to be folded in (staged)
@@ -307,7 +306,7 @@ __device__ __forceinline__ bool beats(float v, int i, float w, int j) {
     return v > w || (v == w && i < j);
 }
 
-constexpr int kListCap = 128;  // entries of a warp's list, four to a lane
+constexpr int kListCap = 64;  // entries of a warp's list, two to a lane
 
 // Sort a warp's list of n entries in shared memory and keep the best k; the
 // number kept. (Out of line: it is called where a list is full and once a row.)
@@ -872,42 +871,42 @@ __global__ void __launch_bounds__(32 * kRowWarps, SHAPE ? 3 : 4)
     if (parts > 1) cluster.sync();  // rank 0 has read this CTA's shared memory
 }
 
-// Many rows: one CTA of up to 24 warps to an SM, each warp with a ring of 4 KB
-// stages of its own that bulk copies fill, so that the copies of the rows to come go on
-// while a row is joined and its best columns are found. TEAM warps share a row (1
-// up to 8 KB, else 4), and the CTA's teams a run of consecutive rows, item by
-// item; g stays in shared memory for an item.
-constexpr int kRingStages = 4;  // at most
-constexpr int kRingVecs = 8;    // vectors of a lane in a stage
-constexpr int kRingBytes = 32 * kRingVecs * 16;
-// Warps of a CTA. Without g 20 of them with 96 registers beat 24 with 80 (16384 x
-// 4096 bf16: 37 us against 51 us), with g it is the other way (16 x 2048 x 2048
-// with a mask and top 4: 101 us against 93 us).
+// Many rows: one CTA of 20 or 28 warps to an SM. Each warp has 4 KB of shared
+// memory that a bulk copy fills with its next piece of a row while it works on the
+// last one in registers, across rows: the copy goes on while a row is joined and
+// its best columns are found. (More stages a warp gained nothing and took the L1
+// cache: 16 x 2048 x 2048 fp32 59 us with one, 65 us with two.) TEAM warps share a
+// row (1 up to 8 KB, else 4), and the CTA's teams a run of consecutive rows, item
+// by item; g stays in shared memory for an item.
+constexpr int kAheadVecs = 8;  // vectors of a lane in a copy
+constexpr int kAheadBytes = 32 * kAheadVecs * 16;
+// Warps of a CTA. Without g 20 with 96 registers beat 28 with 72 (16384 x 4096
+// bf16: 36 us against 54 us), with g it is the other way (16 x 2048 x 2048 with a
+// mask and top 4: 96 us against 86 us).
 template <int SHAPE>
-constexpr int ring_warps() {
-    return SHAPE == kPlain ? 20 : 24;
+constexpr int stream_warps() {
+    return SHAPE == kPlain ? 20 : 28;
 }
 
 template <typename T, int SHAPE, bool TOP, int TEAM>
-__global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const RowProbArgs A) {
+__global__ void __launch_bounds__(stream_warps<SHAPE>() * 32, 1) k_row_stream(const RowProbArgs A) {
     constexpr int V = Vec<T>::n, V2 = V / 2;
-    constexpr int H = 32 / V < kRingVecs ? 32 / V : kRingVecs;  // vectors folded at once
-    constexpr int WARPS = ring_warps<SHAPE>(), TEAMS = WARPS / TEAM;
+    constexpr int H = 32 / V < kAheadVecs ? 32 / V : kAheadVecs;  // vectors folded at once
+    constexpr int WARPS = stream_warps<SHAPE>(), TEAMS = WARPS / TEAM;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int team = warp / TEAM, tw = warp % TEAM;
     __shared__ RowShared<TOP, TEAM> shared[TEAMS];
-    __shared__ uint64_t bars[WARPS][kRingStages];
+    __shared__ uint64_t bars[WARPS];
     RowShared<TOP, TEAM>& sh = shared[team];
-    uint64_t* const full = bars[warp];
-    const int stages = A.stages;
-    uint8_t* const ring = reinterpret_cast<uint8_t*>(staged_g) +
-                          (A.staged ? align16((int)A.M * 4) : 0) + warp * stages * kRingBytes;
+    uint64_t* const full = &bars[warp];
+    uint8_t* const buffer = reinterpret_cast<uint8_t*>(staged_g) +
+                            (A.staged ? align16((int)A.M * 4) : 0) + warp * kAheadBytes;
     auto sync = [&] {
         if (TEAM == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(TEAM * 32) : "memory");
     };
     if (lane == 0) {
-        for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+        mbar_init(full, 1);
         mbar_init_fence();
     }
     __syncwarp();
@@ -918,7 +917,7 @@ __global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const 
     const unsigned N = (unsigned)A.N;
     const int M = (int)A.M, k = A.top_k;
     const float k2 = A.k * kLog2e;
-    const int first = tw * 32 * kRingVecs, step = TEAM * 32 * kRingVecs;
+    const int first = tw * 32 * kAheadVecs, step = TEAM * 32 * kAheadVecs;
     // without g the CTA's rows are one run; with it, runs of an item
     auto run_end = [&](int r) {
         return SHAPE == kPlain ? R1 : (int)min((unsigned)R1, (r / N + 1) * N);
@@ -946,9 +945,8 @@ __global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const 
         left = A.mask_a && !A.mask_a[row] ? 0 : (M - lead) / V - first;
     };
     if (ahead < R1) open(ahead);
-    int issue_at = 0, use_at = 0;  // stages
-    uint32_t phase = 0;            // bit s: the phase to wait for
-    // the copy of the next step into the stage that is free
+    uint32_t phase = 0;  // of `full`
+    // the copy of the next step, once the buffer has been read
     auto issue = [&] {
         while (left <= 0) {
             if (ahead < R1) ahead = next_row(ahead, ahead_end);
@@ -956,15 +954,14 @@ __global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const 
             open(ahead);
         }
         if (lane == 0) {
-            const uint32_t bytes = min(32 * kRingVecs, left) * 16;
-            mbar_expect_tx(&full[issue_at], bytes);
-            bulk_g2s(ring + issue_at * kRingBytes, src, bytes, &full[issue_at]);
+            const uint32_t bytes = min(32 * kAheadVecs, left) * 16;
+            mbar_expect_tx(full, bytes);
+            bulk_g2s(buffer, src, bytes, full);
         }
-        if (++issue_at == stages) issue_at = 0;
         src += step * V;
         left -= step;
     };
-    for (int s = 0; s < stages; ++s) issue();
+    issue();
 
     bool ok = true;
     int end = run_end(R0);
@@ -985,21 +982,21 @@ __global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const 
             Moments mo;
             float best = kNegInf;
             for (int i = first; i < nv; i += step) {
-                if (!mbar_try_wait(&full[use_at], phase >> use_at & 1))
-                    ok = mbar_wait(&full[use_at], phase >> use_at & 1) && ok;
+                if (!mbar_try_wait(full, phase)) ok = mbar_wait(full, phase) && ok;
                 __syncwarp();
-                phase ^= 1u << use_at;
-                const uint4* const p =
-                    reinterpret_cast<const uint4*>(ring + use_at * kRingBytes) + lane;
-                if (++use_at == stages) use_at = 0;
-                const bool whole = i + 32 * kRingVecs <= nv;
+                phase ^= 1;
+                const uint4* const p = reinterpret_cast<const uint4*>(buffer) + lane;
+                const bool whole = i + 32 * kAheadVecs <= nv;
 #pragma unroll
-                for (int h = 0; h < kRingVecs; h += H) {
+                for (int h = 0; h < kAheadVecs; h += H) {
                     uint4 raw[H];
 #pragma unroll
                     for (int q = 0; q < H; ++q) raw[q] = p[(h + q) * 32];
-                    if (h + H == kRingVecs) {
-                        __syncwarp();  // the stage is read
+                    if (h + H == kAheadVecs) {
+                        // the buffer is read: loads that are still on their way would
+                        // otherwise see what the copy brings
+                        fence_async_smem();
+                        __syncwarp();
                         issue();
                     }
                     float2 x[H * V2];
@@ -1039,7 +1036,7 @@ __global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const 
                 top.i = sh.li[tw];
                 top.offer(endv, end_j, k, kNegInf, lane);
                 const float bound = lane_bound<TEAM>(sh, best, k, tw, lane, sync);
-                offer_again<T, SHAPE, kRingVecs>(top, sh.from[tw], best, bound, X, rs,
+                offer_again<T, SHAPE, kAheadVecs>(top, sh.from[tw], best, bound, X, rs,
                                                  lead, nv, first, step, k, lane);
                 if (TEAM == 1 || top.n > 32) top.keep(k, lane);
             }
@@ -1071,9 +1068,8 @@ __global__ void __launch_bounds__(ring_warps<SHAPE>() * 32, 1) k_row_ring(const 
             }
         }
     }
-    // copies that a wait gave up on may still be on their way
-    if (!ok)
-        for (int s = 0; s < stages; ++s) mbar_wait(&full[s], phase >> s & 1, 1u << 12);
+    // a copy that a wait gave up on may still be on its way
+    if (!ok) mbar_wait(full, phase ^ 1, 1u << 16);
 }
 
 constexpr int64_t kStagedMax = 16384;  // columns of g that are held in shared memory
@@ -1125,28 +1121,26 @@ int launch_cta(const RowProbArgs& A, int cluster, cudaStream_t s) {
 }
 
 template <typename T, int SHAPE, bool TOP, int TEAM>
-int launch_ring(RowProbArgs A, cudaStream_t s) {
-    cudaFuncAttributes fa;
-    SK_CUDA(cudaFuncGetAttributes(&fa, k_row_ring<T, SHAPE, TOP, TEAM>));
-    const size_t held = A.staged ? align16((int)A.M * 4) : 0;
-    const size_t stage = (size_t)ring_warps<SHAPE>() * kRingBytes;
-    A.stages = (int)std::min<size_t>(kRingStages, (232448 - fa.sharedSizeBytes - held) / stage);
-    const size_t smem = held + A.stages * stage;
-    const int rc = allow_smem(k_row_ring<T, SHAPE, TOP, TEAM>, smem);
+int launch_stream(const RowProbArgs& A, cudaStream_t s) {
+    constexpr int warps = stream_warps<SHAPE>(), teams = warps / TEAM;
+    const size_t smem = (A.staged ? align16((int)A.M * 4) : 0) + (size_t)warps * kAheadBytes;
+    const int rc = allow_smem(k_row_stream<T, SHAPE, TOP, TEAM>, smem);
     if (rc != SK_OK) return rc;
-    const int64_t rows = A.B * A.N, teams = ring_warps<SHAPE>() / TEAM;
+    const int64_t rows = A.B * A.N;
     const unsigned grid = (unsigned)std::min<int64_t>(148, (rows + teams - 1) / teams);
-    k_row_ring<T, SHAPE, TOP, TEAM><<<grid, ring_warps<SHAPE>() * 32, smem, s>>>(A);
-    SK_LAUNCHED("k_row_ring");
+    k_row_stream<T, SHAPE, TOP, TEAM><<<grid, warps * 32, smem, s>>>(A);
+    SK_LAUNCHED("k_row_stream");
     return SK_OK;
 }
 
 // How the rows are split. Up to 2 KB a warp holds a row in registers and nothing
 // is joined or read twice; a CTA takes at least a row of an item to each warp.
-// Longer rows go to the rings where there are enough to keep them busy (and, with
+// Longer rows are streamed where there are enough to keep 148 CTAs busy (and, with
 // a g that is staged per item, items of some length), else a row takes a CTA, or
 // a cluster of up to 8 where the rows alone leave SMs idle (each with at least
-// one full step of its warps).
+// one full step of its warps). Without g, rows beyond 8 KB stay with a CTA each:
+// its 32 warps an SM hide more than the stream (8192 x 65536 bf16: 183 us against
+// 219 us; 16384 x 4096: 50 us against 36 us).
 template <typename T, int SHAPE, bool TOP>
 int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
     const int64_t bytes = A.M * (int64_t)sizeof(T), rows = A.B * A.N;
@@ -1157,9 +1151,9 @@ int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
                             : launch_held<T, SHAPE, TOP, 4>(A, per, s);
     }
     const bool runs = (SHAPE == kPlain || A.N >= 64) && rows < INT_MAX / 2;
-    if (bytes <= 8192 && rows >= 148 * 16 && runs) return launch_ring<T, SHAPE, TOP, 1>(A, s);
+    if (bytes <= 8192 && rows >= 148 * 16 && runs) return launch_stream<T, SHAPE, TOP, 1>(A, s);
     if (SHAPE != kPlain && bytes > 8192 && rows >= 148 * 4 && runs)
-        return launch_ring<T, SHAPE, TOP, 4>(A, s);
+        return launch_stream<T, SHAPE, TOP, 4>(A, s);
     int cluster = 1;
     while (cluster < 8 && rows * cluster * 2 <= 148 * 4 &&
            bytes > (int64_t)cluster * kRowWarps * 32 * 4 * 16)
@@ -1552,6 +1546,8 @@ int check_rows(const void* X, int dtype, int64_t B, int64_t N, int64_t M, int64_
     if (dtype < SK_FP32 || dtype > SK_FP16) return fail(SK_ERR_ARG, "unknown element type");
     const int rc = check_problem(reinterpret_cast<const float*>(X), B, N, M, epsilon);
     if (rc != SK_OK) return rc;
+    if (!std::isfinite((float)(1.0 / epsilon)))
+        return fail(SK_ERR_ARG, "1 / epsilon is beyond fp32");
     if (M > INT_MAX || N > INT_MAX) return fail(SK_ERR_ARG, "N and M must be below 2^31");
     if (sXm != 1) return fail(SK_ERR_LAYOUT, "the rows must have unit column stride");
     if (sXb < 0 || sXn < 0) return fail(SK_ERR_LAYOUT, "negative strides");

@@ -331,6 +331,45 @@ def test_token_gradient_odd_rows(V):
     assert ((d.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 300 * U32 * p).all()
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("N,M,k", [(2500, 4091, 3), (2500, 1999, 0), (700, 9001, 2)])
+def test_many_rows_give_the_same_every_time(N, M, k, dtype):
+    """Rows that are streamed through shared memory: a copy that overtakes the loads of
+    the last piece would show in some of the runs."""
+    C, g, _, ma, mb = (v.cuda() for v in make(1, N, M, TYPES[dtype], N + M))
+    first = _skb().row_logprobs(C, g, 0.25, None, k, ma, mb)
+    rows = slice(0, None, 97)
+    ref = plain(shaped(C[:, rows].cpu(), g.cpu(), ma[:, rows].cpu(), mb.cpu()), 4.0, k=k)
+    sub = type(first)(*(None if v is None else v[:, rows] for v in (
+        first.lse, first.entropy, first.logprob, first.top_logprob, first.top_index)))
+    check(sub, ref, M, k)
+    for _ in range(20):
+        r = _skb().row_logprobs(C, g, 0.25, None, k, ma, mb)
+        assert torch.equal(r.lse, first.lse) and torch.equal(r.entropy, first.entropy)
+        assert k == 0 or torch.equal(r.top_index, first.top_index)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V", [9, 700, 30000])
+def test_masks_of_the_types_lowest_value(V, dtype):
+    """Logits masked by the lowest finite value, some rows wholly so: those are uniform."""
+    low = torch.finfo(TYPES[dtype]).min
+    x = torch.randn(3, V, generator=torch.Generator().manual_seed(V)).to(TYPES[dtype])
+    x[0, ::2] = low
+    x[1] = low
+    X = x.cuda().requires_grad_()
+    r = _skb().token_logprobs(X, torch.tensor([1, 2, 3]).cuda(), 4)
+    # (shifted by each row's maximum: log 1e4 beside 1e38 is lost in 64 bits, too)
+    ref = plain(x.double() - x.double().amax(1, keepdim=True), 1.0, torch.tensor([1, 2, 3]), 4)
+    for got, want in ((r.entropy, ref["entropy"]), (r.logprob, ref["logprob"])):
+        assert (got.detach().double().cpu() - want).abs().max() < 1e-4
+    assert torch.equal(r.top_index.cpu(), ref["top_index"])
+    d, = torch.autograd.grad(r.logprob.sum(), X)
+    p = ref["p"]
+    p[torch.arange(3), torch.tensor([1, 2, 3])] -= 1
+    assert (d.double().cpu() + p).abs().max() < torch.finfo(TYPES[dtype]).eps
+
+
 def test_same_result_twice_and_under_capture_on_another_stream():
     C, g, t, _, mb = make(2, 700, 200, torch.float32, 8)
     X, G, t, mb = C.cuda().requires_grad_(), g.cuda().requires_grad_(), t.cuda(), mb.cuda()

@@ -154,6 +154,7 @@ _ENTRIES = [
     ("rows type", lambda L: _rows(L, dt=3), ARG),
     ("rows M=0", lambda L: _rows(L, M=0), ARG),
     ("rows eps", lambda L: _rows(L, eps=float("inf")), ARG),
+    ("rows eps tiny", lambda L: _rows(L, eps=1e-45), ARG),
     ("rows strided columns", lambda L: _rows(L, sm=2), LAYOUT),
     ("rows negative stride", lambda L: _rows(L, sn=-8), LAYOUT),
     ("rows misaligned", lambda L: _rows(L, X=_P + 2), LAYOUT),
