@@ -94,6 +94,8 @@ def sum_rows_backward(grad: Tensor, y: Tensor, position: Tensor, offsets: Tensor
 
 def _strides(t: Tensor) -> tuple:
     """Strides of t; an axis of one element has stride 1."""
+    if 1 not in t.shape:
+        return t.stride()
     return tuple(s if n > 1 else 1 for s, n in zip(t.stride(), t.shape))
 
 
@@ -146,10 +148,13 @@ def product(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
         return y
     if not K:
         return y.zero_()
+    se, sk, sn = _strides(w)
+    if N == 1 and K > 1 and sk == 1:
+        sn = K  # one column a group: its K elements are the row
     with T.on(x.device):
         rc = T.lib().sk_grouped_matmul(
-            x.data_ptr(), T.DTYPES[x.dtype], S, K, x.stride(0), w.data_ptr(), E, N,
-            *_strides(w), offsets.data_ptr(), y.data_ptr(), T.stream_of(x.device))
+            x.data_ptr(), T.DTYPES[x.dtype], S, K, x.stride(0), w.data_ptr(), E, N, se, sk,
+            sn, offsets.data_ptr(), y.data_ptr(), T.stream_of(x.device))
         T.check(rc, "sk_grouped_matmul")
     return y
 

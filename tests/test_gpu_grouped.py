@@ -83,7 +83,7 @@ def test_products_and_gradients(S, E, K, N, ends, dtype):
     check(*make(S, E, K, N, dtype, S + K), ends)
 
 
-@pytest.mark.parametrize("K,N", [(1, 1), (7, 3), (33, 65), (64, 77), (1001, 64), (130, 262)])
+@pytest.mark.parametrize("K,N", [(1, 1), (1, 40), (40, 1), (1, 7), (9, 1), (16, 1), (7, 3), (33, 65), (64, 77), (1001, 64), (130, 262)])
 def test_widths_that_are_not_multiples_of_eight(K, N):
     check(*make(150, 3, K, N, "bf16", K), [0, 70, 71, 149])
     check(*make(90, 2, K, N, "fp16", K), [0, 33, 90])

@@ -372,26 +372,31 @@ def test_masks_of_the_types_lowest_value(V, dtype):
 
 def test_same_result_twice_and_under_capture_on_another_stream():
     C, g, t, _, mb = make(2, 700, 200, torch.float32, 8)
-    X, G, t, mb = C.cuda().requires_grad_(), g.cuda().requires_grad_(), t.cuda(), mb.cuda()
+    t, mb = t.cuda(), mb.cuda()
 
-    def step():
+    def step(X, G):
         r = _skb().row_logprobs(X, G, 0.5, t, 3, None, mb)
         d = torch.autograd.grad(r.logprob.sum() + r.top_logprob.sum() + r.entropy.sum(), (X, G))
-        return (r.lse, r.entropy, r.logprob, r.top_index, r.top_logprob) + d
+        return tuple(v.detach() for v in (r.lse, r.entropy, r.logprob, r.top_index,
+                                          r.top_logprob) + d)
 
-    first = [v.detach().clone() for v in step()]
+    def leaves(scale=1.0):
+        return (scale * C).cuda().requires_grad_(), g.cuda().requires_grad_()
+
+    first = step(*leaves())
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
-        for v, w in zip(step(), first):
+        for v, w in zip(step(*leaves()), first):
             assert torch.equal(v, w)
+        held = leaves()  # leaves that no eager graph refers to
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=s):
-            out = step()
+            out = step(*held)
     torch.cuda.synchronize()
     with torch.no_grad():
-        X.copy_(2 * X)
+        held[0].copy_(2 * C)
     graph.replay()
     torch.cuda.synchronize()
-    for v, w in zip(step(), out):
+    for v, w in zip(step(*leaves(2.0)), out):
         assert torch.equal(v, w)
