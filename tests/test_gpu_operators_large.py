@@ -1,0 +1,149 @@
+"""The row, expert and grouped operators where offsets pass 2^31 elements, and side by side
+on two streams and in captured graphs."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+
+
+def _skb():
+    import sinkhorn_b200
+    return sinkhorn_b200
+
+
+def _need(gb):
+    free, _ = torch.cuda.mem_get_info()
+    if free < gb * 1e9:
+        pytest.skip(f"needs {gb} GB of device memory")
+
+
+def test_logits_beyond_2_31_elements():
+    _need(16)
+    skb = _skb()
+    T, V = 36000, 65536
+    x = torch.empty(T, V, device="cuda", dtype=torch.bfloat16)
+    torch.manual_seed(0)
+    for i in range(0, T, 4000):
+        x[i:i + 4000].normal_()
+    t = torch.arange(T, device="cuda") * 13 % V
+    x.requires_grad_()
+    r = skb.token_logprobs(x, t, 3)
+    d, = torch.autograd.grad(r.logprob, x, torch.ones(T, device="cuda"))
+    at = torch.tensor([0, 1, 32767, 32768, 32769, T - 1]).cuda()
+    z = x.detach()[at].double()
+    lp = torch.log_softmax(z, 1)
+    want = lp.gather(1, t[at][:, None])[:, 0]
+    # a lane sums 256 terms of up to (2 * 12 + 4) u each
+    assert (r.logprob.detach()[at] - want).abs().max() < 400 * U32 * 12
+    order = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :3]
+    assert torch.equal(r.top_index[at], order)
+    g = -lp.exp()
+    g.scatter_add_(1, t[at][:, None], torch.ones(6, 1, device="cuda", dtype=torch.float64))
+    assert ((d[at].double() - g).abs() <= 2.0 ** -8 * g.abs() + 500 * U32 * lp.exp()).all()
+
+
+def test_rows_beyond_2_31_elements():
+    _need(22)
+    skb = _skb()
+    T, k, D = 270000, 4, 2048
+    index = (torch.arange(T * k, device="cuda").view(T, k) * 7 + torch.arange(T, device="cuda")[:, None]) % 16
+    d = skb.expert_dispatch(index, 16)
+    x = torch.arange(T, device="cuda").remainder(251).to(torch.bfloat16)[:, None].expand(T, D)
+    rows = skb.dispatch_rows(x, d)
+    token = torch.div(d.order, k, rounding_mode="floor").long()
+    assert torch.equal(rows[:, 0], x[token, 0]) and torch.equal(rows[:, -1], x[token, 0])
+    out = skb.combine_rows(rows, d)
+    # four times a whole number up to 250 is exact in bf16 up to its rounding
+    want = (4.0 * x[:, 0].float()).to(torch.bfloat16)
+    assert torch.equal(out[:, 0], want) and torch.equal(out[:, -1], want)
+
+
+def test_products_beyond_2_31_elements():
+    _need(16)
+    skb = _skb()
+    S, K, N = 540000, 4096, 64
+    x = torch.empty(S, K, device="cuda", dtype=torch.bfloat16)
+    torch.manual_seed(1)
+    for i in range(0, S, 60000):
+        x[i:i + 60000].normal_()
+    w = (torch.randn(3, K, N, device="cuda") / 64).bfloat16()
+    ends = [0, 100, 530000, S]
+    y = skb.grouped_matmul(x, w, torch.tensor(ends, device="cuda"))
+    for r, e in ((0, 0), (99, 0), (100, 1), (529999, 1), (530000, 2), (S - 1, 2)):
+        want = x[r].double() @ w[e].double()
+        size = x[r].double().abs() @ w[e].double().abs()
+        assert ((y[r].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2 * K * U32 * size).all()
+    g = torch.zeros(S, N, device="cuda", dtype=torch.bfloat16)
+    g[S - 5:] = 1.0
+    W = w.clone().requires_grad_()
+    dw, = torch.autograd.grad(skb.grouped_matmul(x, W, torch.tensor(ends, device="cuda")), W, g)
+    want = x[S - 5:].double().sum(0)
+    assert (dw[:2] == 0).all()
+    assert ((dw[2].double() - want[:, None]).abs() <= 2.0 ** -8 * want.abs()[:, None] + 1e-5).all()
+
+
+def _work(skb, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=gen)
+    C, g = r(4, 1500, 700), r(4, 700)
+    x, w = r(3000, 256).bfloat16(), (r(16, 256, 384) / 16).bfloat16()
+    index = torch.randint(0, 16, (3000, 2), device="cuda", generator=gen)
+    leaves = [t.requires_grad_() for t in (C, g, x, w)]
+
+    def step():
+        a = skb.row_logprobs(leaves[0], leaves[1], 0.2, top_k=4)
+        d = skb.expert_dispatch(index, 16)
+        y = skb.grouped_matmul(skb.dispatch_rows(leaves[2], d), leaves[3], d.offsets)
+        o = skb.combine_rows(y, d)
+        l = skb.token_logprobs(o, top_k=3)
+        grads = torch.autograd.grad([a.top_logprob.sum(), a.entropy.sum(), l.entropy.sum()], leaves)
+        return [v.detach() for v in (a.lse, a.top_index, o, l.top_index, *grads)]
+    return step
+
+
+def test_two_streams_at_once():
+    skb = _skb()
+    steps = [_work(skb, s) for s in (1, 2)]
+    torch.cuda.synchronize()
+    alone = [s() for s in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(5):
+        got = []
+        for st, step in zip(streams, steps):
+            with torch.cuda.stream(st):
+                got.append(step())
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_two_captured_graphs_share_nothing():
+    skb = _skb()
+    want = []
+    for s in (3, 4):
+        want.append(_work(skb, s)())
+    graphs, outs, keep = [], [], []
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for s in (3, 4):
+        with torch.cuda.stream(side):
+            step = _work(skb, s)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(step())
+        graphs.append(g)
+        keep.append(step)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, st in zip(graphs, (torch.cuda.Stream(), torch.cuda.Stream())):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
