@@ -55,6 +55,7 @@ struct RowProbArgs {
     int per_cta;            // rows of one item to a CTA
     unsigned groups;        // CTAs of an item
     bool staged;            // each CTA holds g (and mask_b) in shared memory
+    bool vectors;           // every row starts on 16 bytes
     const float* g;         // (B,M) or NULL; -inf where mask_b leaves a column out
     const uint8_t* mask_b;  // (B,M) or NULL: still to be folded in (staged)
     const uint8_t* mask_a;  // (B,N) or NULL
@@ -568,15 +569,15 @@ __device__ __forceinline__ void offer_again(TopList& top, int* from, float best,
     }
 }
 
-// A finished row's outputs, by one warp; its best columns are lv / li [k].
-template <typename T, int SHAPE, bool TOP>
-__device__ __forceinline__ void write_row(const RowProbArgs& A, int64_t row, const T* X,
-                                          const RowShape& rs, const Moments& mo, const float* lv,
-                                          const int* li, int have, int lane) {
+// A finished row's statistics, written by one lane (`writes`); value(t) is x of
+// column t. Returns log s.
+template <typename F>
+__device__ __forceinline__ float write_stats(const RowProbArgs& A, int64_t row, const Moments& mo,
+                                             bool writes, F value) {
     // an empty row keeps s = 0; a row of NaN alone has s = NaN
     const bool none = mo.m == kNegInf && mo.s == 0.f;
     const float logs = none ? 0.f : logf(mo.s);
-    if (lane == 0) {
+    if (writes) {
         if (A.stats) A.stats[row] = make_float2(none ? kNegInf : mo.m, logs);
         if (A.lse) A.lse[row] = none ? kNegInf : fmaf(mo.m, A.k, logs);
         if (A.entropy) A.entropy[row] = none ? 0.f : logs - kLn2 * (mo.u / mo.s);
@@ -584,17 +585,31 @@ __device__ __forceinline__ void write_row(const RowProbArgs& A, int64_t row, con
             const int64_t t = A.targets[row];
             float lp = 0.f;
             if (t >= A.M) lp = NAN;
-            else if (t >= 0) {
-                const float v = none ? kNegInf : shaped<SHAPE>(widen(X[t]), rs, t);
-                lp = none ? kNegInf : fmaf(v - mo.m, A.k, -logs);
-            }
+            else if (t >= 0) lp = none ? kNegInf : fmaf(value(t) - mo.m, A.k, -logs);
             A.logprob[row] = lp;
         }
     }
+    return logs;
+}
+
+// Its `at`-th best column; `held` is false where there are fewer.
+__device__ __forceinline__ void write_best(const RowProbArgs& A, int64_t row, const Moments& mo,
+                                           float logs, int at, bool held, float v, int i) {
+    A.top_lp[row * A.top_k + at] = held ? fmaf(v - mo.m, A.k, -logs) : kNegInf;
+    A.top_idx[row * A.top_k + at] = held ? i : -1;
+}
+
+// A finished row's outputs, by one warp; its best columns are lv / li [k].
+template <typename T, int SHAPE, bool TOP>
+__device__ __forceinline__ void write_row(const RowProbArgs& A, int64_t row, const T* X,
+                                          const RowShape& rs, const Moments& mo, const float* lv,
+                                          const int* li, int have, int lane) {
+    const float logs = write_stats(A, row, mo, lane == 0, [&](int64_t t) {
+        return shaped<SHAPE>(widen(X[t]), rs, t);
+    });
     if (TOP && lane < A.top_k) {
         const bool held = lane < have && li[lane] >= 0;
-        A.top_lp[row * A.top_k + lane] = held ? fmaf(lv[lane] - mo.m, A.k, -logs) : kNegInf;
-        A.top_idx[row * A.top_k + lane] = held ? li[lane] : -1;
+        write_best(A, row, mo, logs, lane, held, held ? lv[lane] : 0.f, held ? li[lane] : -1);
     }
 }
 
@@ -606,6 +621,132 @@ __device__ __forceinline__ float row_ends(const T* X, const RowShape& rs, int le
     column = lane < 16 ? lane : tail + lane - 16;
     const bool on = lane < 16 ? lane < lead : column < M;
     return on ? shaped<SHAPE>(widen(X[column]), rs, column) : kNegInf;
+}
+
+constexpr int kGroupLanes = 8;  // lanes of a row in k_row_group
+constexpr int kGroupTop = 8;    // most of its best columns: one to a lane
+
+// Rows of up to 8 * P columns, as a router's experts: 8 lanes to a row, P values
+// each, four rows to a warp at once, since joining 32 lanes costs such rows more
+// than reading them. A lane's columns are the same in every row of an item, so g
+// and its mask stay in registers. A best column costs a maximum over the lanes'
+// own best ones, after which the lane that held it looks for its next.
+// 16 x 32768 x 64 fp32 with g, best 2: 76 us (335 us by a warp to a row); 4 x 8192:
+// 8 us (27 us). 32768 x 128 bf16, best 8: 22 us (42 us).
+template <typename T, int SHAPE, bool TOP, int P>
+__global__ void __launch_bounds__(32 * kRowWarps, P == 8 ? 4 : 3)
+    k_row_group(const RowProbArgs A) {
+    constexpr int V = Vec<T>::n, Q = P / V, G = kGroupLanes;
+    constexpr int kGroups = 32 * kRowWarps / G;
+    static_assert(P % V == 0, "whole vectors");
+    const int gl = threadIdx.x % G, group = threadIdx.x / G;
+    const unsigned item = blockIdx.x / A.groups;
+    const int64_t b = item, r0 = (int64_t)(blockIdx.x - item * A.groups) * A.per_cta;
+    const int64_t r1 = min(A.N, r0 + A.per_cta);
+    const T* const Xb = reinterpret_cast<const T*>(A.X) + b * A.sXb;
+    const int M = (int)A.M, k = A.top_k;
+    const float k2 = A.k * kLog2e;
+    // column of the lane's value e
+    auto column = [&](int e) { return (e / V * G + gl) * V + e % V; };
+    auto g_at = [&](int64_t j) {
+        const float v = A.g ? A.g[b * M + j] : 0.f;
+        return SHAPE == kMasked && A.mask_b && !A.mask_b[b * M + j] ? kNegInf : v;
+    };
+    uint4 raw[Q];
+    bool off = true;  // a row behind the last, or left out by mask_a
+    auto load = [&](int64_t r) {
+        off = r >= r1 || (A.mask_a && !A.mask_a[b * A.N + r]);
+        const T* const X = Xb + r * A.sXn;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int j = column(q * V);
+            raw[q] = make_uint4(0, 0, 0, 0);
+            if (off || j >= M) continue;
+            if (A.vectors && j + V <= M) {
+                raw[q] = ld_stream16(X + j);
+            } else {
+                T t[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) t[e] = j + e < M ? X[j + e] : T(0.f);
+                memcpy(&raw[q], t, 16);
+            }
+        }
+    };
+    load(r0 + group);
+    float2 g[P / 2];  // -inf behind the last column
+#pragma unroll
+    for (int e = 0; e < P; e += 2) {
+        const int j = column(e);
+        g[e / 2].x = j >= M ? kNegInf : SHAPE == kPlain ? 0.f : g_at(j);
+        g[e / 2].y = j + 1 >= M ? kNegInf : SHAPE == kPlain ? 0.f : g_at(j + 1);
+    }
+
+    // every lane of a warp stays to the end: the groups share its shuffles
+    for (int64_t r = r0 + group; r - group < r1; r += kGroups) {
+        const int64_t row = b * A.N + r;
+        const bool out = off, in = r < r1;
+        float2 x[P / 2];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) unpack2(raw[q], x + q * (V / 2), (const T*)nullptr);
+        load(r + kGroups);
+        float cm = kNegInf;
+#pragma unroll
+        for (int e = 0; e < P / 2; ++e) {
+            if (SHAPE != kPlain) x[e] = __ffma2_rn(x[e], make_float2(A.sign, A.sign), g[e]);
+            // masked columns, whatever was read there (and what is no column, where
+            // the sum with g has not made it so)
+            if (out || (SHAPE != kAffine && g[e].x == kNegInf)) x[e].x = kNegInf;
+            if (out || (SHAPE != kAffine && g[e].y == kNegInf)) x[e].y = kNegInf;
+            cm = fmaxf(cm, fmaxf(x[e].x, x[e].y));
+        }
+        Moments mo;
+        mo.fold<true>(x, cm, k2);
+        float m = mo.m;
+#pragma unroll
+        for (int d = G / 2; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        mo.move_to(m, k2);
+#pragma unroll
+        for (int d = G / 2; d > 0; d /= 2) {
+            mo.s += __shfl_xor_sync(0xffffffffu, mo.s, d);
+            mo.u += __shfl_xor_sync(0xffffffffu, mo.u, d);
+        }
+
+        float bv = kNegInf;  // the lane's entry of the best k
+        int bj = INT_MAX;
+        if constexpr (TOP) {
+            for (int i = 0; i < k; ++i) {
+                float v = kNegInf;  // the lane's best value that is left
+                int j = INT_MAX;
+#pragma unroll
+                for (int e = 0; e < P / 2; ++e) {
+                    if (x[e].x > v) v = x[e].x, j = column(2 * e);
+                    if (x[e].y > v) v = x[e].y, j = column(2 * e + 1);
+                }
+                float w = v;
+                int wj = j;
+#pragma unroll
+                for (int d = G / 2; d > 0; d /= 2) {
+                    const float ov = __shfl_xor_sync(0xffffffffu, w, d);
+                    const int oj = __shfl_xor_sync(0xffffffffu, wj, d);
+                    if (beats(ov, oj, w, wj)) w = ov, wj = oj;
+                }
+                if (gl == i) bv = w, bj = wj;
+                if (j == wj) {  // this lane's: not again (INT_MAX: none is left)
+#pragma unroll
+                    for (int e = 0; e < P / 2; ++e) {
+                        if (column(2 * e) == wj) x[e].x = kNegInf;
+                        if (column(2 * e + 1) == wj) x[e].y = kNegInf;
+                    }
+                }
+            }
+        }
+        if (!in) continue;
+        const float logs = write_stats(A, row, mo, gl == 0, [&](int64_t t) {
+            const float v = widen(Xb[r * A.sXn + t]);
+            return SHAPE == kPlain ? v : shaped1<SHAPE>(v, g_at(t), A.sign);
+        });
+        if (TOP && gl < k) write_best(A, row, mo, logs, gl, bj != INT_MAX, bv, bj);
+    }
 }
 
 // Short rows: a warp to a row, which is at most U vectors of 16 bytes a lane,
@@ -1103,6 +1244,22 @@ int launch_held(RowProbArgs A, int per_cta, cudaStream_t s) {
     return SK_OK;
 }
 
+template <typename T, int SHAPE, bool TOP, int P>
+int launch_group(RowProbArgs A, cudaStream_t s) {
+    constexpr int groups = 32 * kRowWarps / kGroupLanes;
+    // one wave of CTAs, 4 an SM, then more rows each
+    const int64_t want = (A.B * A.N / (148 * 4) + groups - 1) / groups * groups;
+    A.per_cta = (int)std::max<int64_t>(groups, std::min<int64_t>(want, 8 * groups));
+    A.groups = (unsigned)((A.N + A.per_cta - 1) / A.per_cta);
+    const int64_t ctas = A.groups * A.B;
+    if (ctas > INT_MAX) return fail(SK_ERR_ARG, "B * N is too large");
+    const int64_t align = 16 / (int64_t)sizeof(T);
+    A.vectors = (uintptr_t)A.X % 16 == 0 && A.sXb % align == 0 && A.sXn % align == 0;
+    k_row_group<T, SHAPE, TOP, P><<<(unsigned)ctas, 32 * kRowWarps, 0, s>>>(A);
+    SK_LAUNCHED("k_row_group");
+    return SK_OK;
+}
+
 template <typename T, int SHAPE, bool TOP>
 int launch_cta(const RowProbArgs& A, int cluster, cudaStream_t s) {
     const int64_t ctas = A.B * A.N * cluster;
@@ -1149,6 +1306,9 @@ int launch_stream(const RowProbArgs& A, cudaStream_t s) {
 template <typename T, int SHAPE, bool TOP>
 int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
     const int64_t bytes = A.M * (int64_t)sizeof(T), rows = A.B * A.N;
+    if (A.M <= 16 * kGroupLanes && A.top_k <= kGroupTop)
+        return A.M <= 8 * kGroupLanes ? launch_group<T, SHAPE, TOP, 8>(A, s)
+                                      : launch_group<T, SHAPE, TOP, 16>(A, s);
     if (bytes <= 2048) {
         const int64_t want = rows / (148 * 24) / kRowWarps * kRowWarps;
         const int per = (int)std::max<int64_t>(kRowWarps, std::min<int64_t>(want, 32));
@@ -1200,7 +1360,7 @@ int fold_mask(const float** g, const uint8_t* mask_b, int64_t BM, void* workspac
 // for dg: a CTA takes a tile of columns and a band of rows, its row constants
 // in shared memory, so that a thread's columns stay its own and dg needs no
 // atomics (bands are summed in a fixed order by a second kernel). One read and one
-// write, bound by DRAM: 8192 x 65536 bf16 373 us, 5.8 TB/s, 88% of a copy.
+// write, bound by DRAM: 8192 x 65536 bf16 357 us, 6.0 TB/s, 92% of a copy.
 
 struct RowProbBwdArgs {
     const void* X;
@@ -1290,6 +1450,18 @@ __global__ void __launch_bounds__(kBwdThreads, 4) k_row_probs_bwd(const RowProbB
 
         for (int64_t rb0 = r0; rb0 < r1; rb0 += kBwdRows) {
             const int nr = (int)min((int64_t)kBwdRows, r1 - rb0);
+            // (32-bit columns and stepped rows: the kernel is bound by instructions)
+            const T* X = Xb + (rb0 + cy) * A.sXn;
+            T* D = A.dX ? Db + (rb0 + cy) * A.M : nullptr;
+            const int64_t x_step = ty * A.sXn, d_step = A.dX ? ty * A.M : 0;
+            uint4 raw[U];
+            auto load = [&](const T* X) {
+                const unsigned j = (COLS ? 0 : (unsigned)row_lead(X, A.M)) + col0;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (j + u * next_vec + V <= M) raw[u] = ld_stream16(X + j + u * next_vec);
+            };
+            if (VEC && cy < nr) load(X);  // on their way beside the rows' constants
             __syncthreads();  // the last rows' constants and sums are read
             for (int r = threadIdx.x; r < nr; r += kBwdThreads) {
                 const int64_t row = b * A.N + rb0 + r;
@@ -1324,6 +1496,7 @@ __global__ void __launch_bounds__(kBwdThreads, 4) k_row_probs_bwd(const RowProbB
                     }
                     float t = q.at;
                     if (TOP)
+#pragma unroll 4
                         for (int j = 0; j < A.top_k; ++j)
                             if (A.top_idx[row * A.top_k + j] >= 0)
                                 t += A.g_top[row * A.top_k + j];
@@ -1334,18 +1507,6 @@ __global__ void __launch_bounds__(kBwdThreads, 4) k_row_probs_bwd(const RowProbB
                 rc[r] = q;
             }
             __syncthreads();
-            // (32-bit columns and stepped rows: the kernel is bound by instructions)
-            const T* X = Xb + (rb0 + cy) * A.sXn;
-            T* D = A.dX ? Db + (rb0 + cy) * A.M : nullptr;
-            const int64_t x_step = ty * A.sXn, d_step = A.dX ? ty * A.M : 0;
-            uint4 raw[U];
-            auto load = [&](const T* X) {
-                const unsigned j = (COLS ? 0 : (unsigned)row_lead(X, A.M)) + col0;
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (j + u * next_vec + V <= M) raw[u] = ld_stream16(X + j + u * next_vec);
-            };
-            if (VEC && cy < nr) load(X);
             for (int r = cy; r < nr; r += ty, X += x_step, D += d_step) {
                 const RowConst q = rc[r];
                 const int64_t row = b * A.N + rb0 + r;
@@ -1501,14 +1662,18 @@ __global__ void __launch_bounds__(1024) k_band_sum(const float* partial, float* 
     }
 }
 
-// Bands of the backward: enough CTAs for eight to an SM, whole groups of rows.
+// Bands of the backward: CTAs in whole waves of 4 to an SM. Column sums take one
+// wave, since each band is a row of partials (4 x 8192 x 64 fp32: 13 us, with two
+// waves 19 us); without them a band is at most the rows that are held at once (8192 x
+// 65536 bf16: 357 us in four waves, 370 us in 3.5).
 void bwd_bands(int64_t B, int64_t N, int64_t M, bool cols, int elem, int64_t* bands,
                int64_t* band_rows) {
+    constexpr int64_t wave = 148 * 4;
     const int64_t tile = (int64_t)kBwdThreads * kBwdVecs * (16 / elem);
     const int64_t tiles = std::max<int64_t>(1, (M + tile - 1) / tile) * B;
-    int64_t want = std::max<int64_t>(1, 148 * 8 / std::max<int64_t>(1, tiles));
-    // without column sums bands are free; with them each costs a row of partials
-    if (!cols) want = std::max<int64_t>(want, (N + kBwdRows - 1) / kBwdRows);
+    const int64_t few = cols ? 1 : (N + kBwdRows - 1) / kBwdRows;
+    const int64_t waves = std::max<int64_t>(1, (tiles * few + wave - 1) / wave);
+    const int64_t want = std::max<int64_t>(few, cols && waves > 1 ? 1 : waves * wave / tiles);
     const int64_t br = std::max<int64_t>((N + want - 1) / want, 1);
     *bands = (N + br - 1) / br;
     *band_rows = br;

@@ -171,6 +171,45 @@ def test_ties_go_to_the_lowest_column():
         check(r, plain(x.double(), 1.0, k=32), V, 32)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("B,N,M,k", [(1, 5001, 2, 2), (70, 1, 8, 8), (3, 333, 31, 1),
+                                     (2, 2500, 63, 7), (1, 40, 64, 0), (1, 6, 64, 8),
+                                     (1, 1700, 65, 8), (2, 31, 100, 3), (2, 33, 127, 8),
+                                     (1, 21000, 128, 2), (1, 65, 129, 8), (1, 65, 128, 9)])
+def test_short_rows(B, N, M, k, dtype):
+    # rows that start anywhere, with a potential and masks, and as they are
+    C, g, t, ma, mb = make(B, N, M + 3, TYPES[dtype], 100 * M + k, spread=3.0)
+    C = C[..., 2:2 + M] if N % 2 else C[..., :M].contiguous()
+    g, mb, t = g[:, :M], mb[:, :M], t.clamp(max=M - 1)
+    on = C.cuda() if N % 2 == 0 else torch.cat([C, C, C], 2).cuda()[..., M:2 * M]
+    r = _skb().row_logprobs(on, g.cuda(), 0.25, t.cuda(), k, ma.cuda(), mb.cuda())
+    check(r, plain(shaped(C, g, ma, mb), 4.0, t.reshape(-1), k), M, k)
+    r = _skb().row_logprobs(on, g.cuda(), 0.25, t.cuda(), k)
+    check(r, plain(shaped(C, g), 4.0, t.reshape(-1), k), M, k)
+    r = _skb().token_logprobs(on, t.cuda(), k)
+    check(r, plain(C.double().reshape(-1, M), 1.0, t.reshape(-1), k), M, k)
+
+
+def test_short_rows_of_equal_values_and_of_few():
+    x = torch.zeros(6, 61)
+    x[1] = -0.0
+    x[1, 5::2] = 0.0
+    x[2] = torch.arange(61) // 10
+    x[3] = -math.inf
+    x[4] = -math.inf
+    x[4, 60] = x[4, 3] = 1.0
+    x[5, :30] = -math.inf
+    r = _skb().token_logprobs(x.cuda(), top_k=8)
+    check(r, plain(x.double(), 1.0, k=8), 61, 8)
+    x[2, 7] = math.nan
+    x[5] = math.nan
+    r = _skb().token_logprobs(x.cuda(), top_k=8)
+    assert r.lse[[2, 5]].isnan().all() and r.entropy[[2, 5]].isnan().all()
+    assert torch.isfinite(r.lse[[0, 1, 4]]).all() and (r.lse[3] == -math.inf)
+    assert (r.top_index[2] == torch.arange(60, 61).cuda()).any() and (r.top_index[2] != 7).all()
+    assert (r.top_index[5] == -1).all()
+
+
 @pytest.mark.parametrize("V", [100, 5000, 40000])
 def test_sorted_rows(V):
     up = torch.linspace(-3, 3, V).repeat(3, 1)
