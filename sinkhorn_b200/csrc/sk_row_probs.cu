@@ -623,20 +623,19 @@ __device__ __forceinline__ float row_ends(const T* X, const RowShape& rs, int le
     return on ? shaped<SHAPE>(widen(X[column]), rs, column) : kNegInf;
 }
 
-constexpr int kGroupLanes = 8;  // lanes of a row in k_row_group
-constexpr int kGroupTop = 8;    // most of its best columns: one to a lane
+constexpr int kGroupTop = 8;  // most best columns in k_row_group: one to a lane
 
-// Rows of up to 8 * P columns, as a router's experts: 8 lanes to a row, P values
-// each, four rows to a warp at once, since joining 32 lanes costs such rows more
+// Rows of up to G * P columns, as a router's experts: G lanes to a row, P values
+// each, 32 / G rows to a warp at once, since joining 32 lanes costs such rows more
 // than reading them. A lane's columns are the same in every row of an item, so g
 // and its mask stay in registers. A best column costs a maximum over the lanes'
 // own best ones, after which the lane that held it looks for its next.
 // 16 x 32768 x 64 fp32 with g, best 2: 76 us (335 us by a warp to a row); 4 x 8192:
 // 8 us (27 us). 32768 x 128 bf16, best 8: 22 us (42 us).
-template <typename T, int SHAPE, bool TOP, int P>
+template <typename T, int SHAPE, bool TOP, int P, int G>
 __global__ void __launch_bounds__(32 * kRowWarps, P == 8 ? 4 : 3)
     k_row_group(const RowProbArgs A) {
-    constexpr int V = Vec<T>::n, Q = P / V, G = kGroupLanes;
+    constexpr int V = Vec<T>::n, Q = P / V;
     constexpr int kGroups = 32 * kRowWarps / G;
     static_assert(P % V == 0, "whole vectors");
     const int gl = threadIdx.x % G, group = threadIdx.x / G;
@@ -1244,9 +1243,9 @@ int launch_held(RowProbArgs A, int per_cta, cudaStream_t s) {
     return SK_OK;
 }
 
-template <typename T, int SHAPE, bool TOP, int P>
+template <typename T, int SHAPE, bool TOP, int P, int G>
 int launch_group(RowProbArgs A, cudaStream_t s) {
-    constexpr int groups = 32 * kRowWarps / kGroupLanes;
+    constexpr int groups = 32 * kRowWarps / G;
     // one wave of CTAs, 4 an SM, then more rows each
     const int64_t want = (A.B * A.N / (148 * 4) + groups - 1) / groups * groups;
     A.per_cta = (int)std::max<int64_t>(groups, std::min<int64_t>(want, 8 * groups));
@@ -1255,7 +1254,7 @@ int launch_group(RowProbArgs A, cudaStream_t s) {
     if (ctas > INT_MAX) return fail(SK_ERR_ARG, "B * N is too large");
     const int64_t align = 16 / (int64_t)sizeof(T);
     A.vectors = (uintptr_t)A.X % 16 == 0 && A.sXb % align == 0 && A.sXn % align == 0;
-    k_row_group<T, SHAPE, TOP, P><<<(unsigned)ctas, 32 * kRowWarps, 0, s>>>(A);
+    k_row_group<T, SHAPE, TOP, P, G><<<(unsigned)ctas, 32 * kRowWarps, 0, s>>>(A);
     SK_LAUNCHED("k_row_group");
     return SK_OK;
 }
@@ -1295,8 +1294,11 @@ int launch_stream(const RowProbArgs& A, cudaStream_t s) {
     return SK_OK;
 }
 
-// How the rows are split. Up to 2 KB a warp holds a row in registers and nothing
-// is joined or read twice; a CTA takes at least a row of an item to each warp.
+// How the rows are split. Up to 512 columns several lanes hold a row, as long as the
+// best k are few: each costs a scan of the lanes' values (32768 x 512 fp32 with
+// g, none: 22 us against 28 us by a warp to a row; best 8: 87 us against 54 us; 256
+// columns, best 8: 46 us against 51 us). Other rows up to 2 KB are held by a warp and
+// nothing is joined or read twice; a CTA takes at least a row of an item to each warp.
 // Longer rows are streamed where there are enough to keep 148 CTAs busy (and, with
 // a g that is staged per item, items of some length), else a row takes a CTA, or
 // a cluster of up to 8 where the rows alone leave SMs idle (each with at least
@@ -1306,9 +1308,12 @@ int launch_stream(const RowProbArgs& A, cudaStream_t s) {
 template <typename T, int SHAPE, bool TOP>
 int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
     const int64_t bytes = A.M * (int64_t)sizeof(T), rows = A.B * A.N;
-    if (A.M <= 16 * kGroupLanes && A.top_k <= kGroupTop)
-        return A.M <= 8 * kGroupLanes ? launch_group<T, SHAPE, TOP, 8>(A, s)
-                                      : launch_group<T, SHAPE, TOP, 16>(A, s);
+    if (A.M <= (A.top_k <= 2 ? 512 : 256) && A.top_k <= kGroupTop) {
+        if (A.M <= 64) return launch_group<T, SHAPE, TOP, 8, 8>(A, s);
+        if (A.M <= 128) return launch_group<T, SHAPE, TOP, 16, 8>(A, s);
+        if (A.M <= 256) return launch_group<T, SHAPE, TOP, 16, 16>(A, s);
+        return launch_group<T, SHAPE, TOP, 16, 32>(A, s);
+    }
     if (bytes <= 2048) {
         const int64_t want = rows / (148 * 24) / kRowWarps * kRowWarps;
         const int per = (int)std::max<int64_t>(kRowWarps, std::min<int64_t>(want, 32));

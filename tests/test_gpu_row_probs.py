@@ -175,7 +175,9 @@ def test_ties_go_to_the_lowest_column():
 @pytest.mark.parametrize("B,N,M,k", [(1, 5001, 2, 2), (70, 1, 8, 8), (3, 333, 31, 1),
                                      (2, 2500, 63, 7), (1, 40, 64, 0), (1, 6, 64, 8),
                                      (1, 1700, 65, 8), (2, 31, 100, 3), (2, 33, 127, 8),
-                                     (1, 21000, 128, 2), (1, 65, 129, 8), (1, 65, 128, 9)])
+                                     (1, 21000, 128, 2), (1, 65, 129, 8), (1, 65, 128, 9),
+                                     (2, 1111, 200, 6), (1, 40, 256, 8), (3, 33, 257, 2),
+                                     (1, 700, 511, 1), (2, 10, 512, 2), (1, 9, 512, 3)])
 def test_short_rows(B, N, M, k, dtype):
     # rows that start anywhere, with a potential and masks, and as they are
     C, g, t, ma, mb = make(B, N, M + 3, TYPES[dtype], 100 * M + k, spread=3.0)
