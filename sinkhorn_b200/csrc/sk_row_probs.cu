@@ -1021,7 +1021,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, SHAPE ? 3 : 4)
 // last one in registers, across rows: the copy goes on while a row is joined and
 // its best columns are found. (More stages a warp gained nothing and took the L1
 // cache: 16 x 2048 x 2048 fp32 59 us with one, 65 us with two.) TEAM warps share a
-// row (1 up to 8 KB, else 4), and the CTA's teams a run of consecutive rows, item
+// row (1 up to 16 KB, else 4), and the CTA's teams a run of consecutive rows, item
 // by item; g stays in shared memory for an item.
 constexpr int kAheadVecs = 8;  // vectors of a lane in a copy
 constexpr int kAheadBytes = 32 * kAheadVecs * 16;
@@ -1300,11 +1300,13 @@ int launch_stream(const RowProbArgs& A, cudaStream_t s) {
 // columns, best 8: 46 us against 51 us). Other rows up to 2 KB are held by a warp and
 // nothing is joined or read twice; a CTA takes at least a row of an item to each warp.
 // Longer rows are streamed where there are enough to keep 148 CTAs busy (and, with
-// a g that is staged per item, items of some length), else a row takes a CTA, or
-// a cluster of up to 8 where the rows alone leave SMs idle (each with at least
-// one full step of its warps). Without g, rows beyond 8 KB stay with a CTA each:
-// its 32 warps an SM hide more than the stream (8192 x 65536 bf16: 183 us against
-// 219 us; 16384 x 4096: 50 us against 36 us).
+// a g that is staged per item, items of some length): up to 16 KB by a warp each
+// (16384 x 8192 bf16: 61 us, by four 83 us, by a CTA each 88 us; with the best 5 90,
+// 129 and 151 us; with the best 20 165, 160 and 176 us), beyond that by four. Else a
+// row takes a CTA, or a cluster of up to 8 where the rows alone leave SMs idle (each
+// with at least one full step of its warps). Without g, rows beyond 16 KB stay with a
+// CTA each: its 32 warps an SM hide more than the stream (8192 x 65536 bf16: 183 us
+// against 206 us by a warp and 219 us by four).
 template <typename T, int SHAPE, bool TOP>
 int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
     const int64_t bytes = A.M * (int64_t)sizeof(T), rows = A.B * A.N;
@@ -1321,7 +1323,7 @@ int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
                             : launch_held<T, SHAPE, TOP, 4>(A, per, s);
     }
     const bool runs = (SHAPE == kPlain || A.N >= 64) && rows < INT_MAX / 2;
-    if (bytes <= 8192 && rows >= 148 * 16 && runs) return launch_stream<T, SHAPE, TOP, 1>(A, s);
+    if (bytes <= 16384 && rows >= 148 * 16 && runs) return launch_stream<T, SHAPE, TOP, 1>(A, s);
     if (SHAPE != kPlain && bytes > 8192 && rows >= 148 * 4 && runs)
         return launch_stream<T, SHAPE, TOP, 4>(A, s);
     int cluster = 1;
