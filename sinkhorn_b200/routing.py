@@ -15,9 +15,9 @@ import torch
 from torch import Tensor
 
 from . import _tensors as T
-from .experts import (ExpertDispatch, combine_rows, dispatch_rows, expert_dispatch,
-                      grouped_matmul)
-from .logprobs import RowLogprobs, row_logprobs
+from .experts import (MAX_EXPERTS, ExpertDispatch, combine_rows, dispatch_rows,
+                      expert_dispatch, grouped_matmul)
+from .logprobs import MAX_TOP_K, RowLogprobs, row_logprobs
 from .sinkhorn import sinkhorn
 
 
@@ -62,9 +62,13 @@ def sinkhorn_route(scores: Tensor, top_k: int = 1, epsilon: float = 0.1,
     t, E = scores.shape
     if t == 0 or E == 0:
         raise ValueError("scores must hold at least one token and one expert")
-    if not 1 <= top_k <= E:
-        raise ValueError(f"top_k must lie between 1 and {E}, got {top_k}")
+    if E > MAX_EXPERTS:
+        raise ValueError(f"scores must have up to {MAX_EXPERTS} experts, got {E}")
+    if not 1 <= top_k <= min(E, MAX_TOP_K):
+        raise ValueError(f"top_k must lie between 1 and {min(E, MAX_TOP_K)}, got {top_k}")
     if mask is not None:
+        if not isinstance(mask, Tensor):
+            raise TypeError("mask must be a torch.Tensor or None")
         if tuple(mask.shape) != (t,):
             raise ValueError(f"mask must have shape {(t,)}, got {tuple(mask.shape)}")
         mask = mask.reshape(1, t)
@@ -91,12 +95,24 @@ def sinkhorn_experts(x: Tensor, scores: Tensor, w_in: Tensor, w_out: Tensor, top
     float16; scores (T, E). Differentiable in x, scores, w_in and w_out. Further arguments
     go to ``sinkhorn_route``. Returns (out, route).
     """
-    T.check_cuda(x, "x")
-    route = sinkhorn_route(scores, top_k, epsilon, mask, **solver)
-    if x.dim() != 2 or x.shape[0] != scores.shape[0]:
-        raise ValueError(f"x must be 2D with {scores.shape[0]} rows, got {tuple(x.shape)}")
+    for name, t, dims in (("x", x, 2), ("scores", scores, 2), ("w_in", w_in, 3),
+                          ("w_out", w_out, 3)):
+        T.check_cuda(t, name)
+        if t.dim() != dims:
+            raise ValueError(f"{name} must be {dims}D, got {t.dim()}D")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x is on {x.device}")
+        if name != "scores":
+            T.check_dtype(t, name, (torch.bfloat16, torch.float16))
+            if t.dtype != x.dtype:
+                raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}: they must have one type")
+    if x.shape[0] != scores.shape[0]:
+        raise ValueError(f"x must have {scores.shape[0]} rows, got {x.shape[0]}")
     if w_in.shape[0] != scores.shape[1] or w_out.shape[0] != scores.shape[1]:
         raise ValueError(f"w_in and w_out must hold {scores.shape[1]} experts")
+    if w_in.shape[1] != x.shape[1]:
+        raise ValueError(f"x has {x.shape[1]} columns, w_in has {w_in.shape[1]} rows")
+    route = sinkhorn_route(scores, top_k, epsilon, mask, **solver)
     d = route.dispatch
     h = activation(grouped_matmul(dispatch_rows(x, d), w_in, d.offsets))
     return combine_rows(grouped_matmul(h, w_out, d.offsets), d, route.gates), route

@@ -73,6 +73,13 @@ def _checked():
     d = skb.ExpertDispatch(_on(6, dtype=i32), _on(3, 2, dtype=i32), _on(5, dtype=i32))
     x, w, o = _on(6, 8, dtype=bf), _on(2, 8, 4, dtype=bf), _on(3, dtype=i32)
     g = skb.grouped_matmul
+    x16 = _on(3, 8, dtype=bf)
+
+    def layer(x, w_in=None, w_out=None):
+        w_in = _on(4, 8, 6, dtype=bf) if w_in is None else w_in
+        w_out = _on(4, 6, 8, dtype=bf) if w_out is None else w_out
+        return skb.sinkhorn_experts(x, _on(3, 4), w_in, w_out)
+
     return [
         ("top_k", lambda: skb.row_logprobs(C, top_k=5), ValueError, "top_k"),
         ("top_k 33", lambda: skb.token_logprobs(L, top_k=33), ValueError, "32"),
@@ -119,6 +126,19 @@ def _checked():
         ("route mask", lambda: skb.sinkhorn_route(_on(3, 4), 1, mask=_on(4, dtype=torch.bool)),
          ValueError, "mask"),
         ("route empty", lambda: skb.sinkhorn_route(_on(0, 4)), ValueError, "at least one"),
+        ("route width", lambda: skb.sinkhorn_route(_on(3, 1025)), ValueError, "1024"),
+        ("route many", lambda: skb.sinkhorn_route(_on(3, 64), 33), ValueError, "top_k"),
+        ("route mask list", lambda: skb.sinkhorn_route(_on(3, 4), 1, mask=[1, 1, 1]), TypeError,
+         "mask"),
+        ("layer types", lambda: layer(_on(3, 8)), TypeError, "x must be"),
+        ("layer mixed", lambda: layer(x16, w_in=_on(4, 8, 6, dtype=torch.float16)), TypeError,
+         "one type"),
+        ("layer weights", lambda: layer(x16, w_out=[1]), TypeError, "w_out"),
+        ("layer weights 2D", lambda: layer(x16, w_in=_on(8, 6, dtype=bf)), ValueError, "3D"),
+        ("layer rows", lambda: layer(_on(2, 8, dtype=bf)), ValueError, "3 rows"),
+        ("layer experts", lambda: layer(x16, w_out=_on(5, 6, 8, dtype=bf)), ValueError,
+         "4 experts"),
+        ("layer width", lambda: layer(_on(3, 7, dtype=bf)), ValueError, "7 columns"),
     ]
 
 
