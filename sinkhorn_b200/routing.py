@@ -51,7 +51,8 @@ def sinkhorn_route(scores: Tensor, top_k: int = 1, epsilon: float = 0.1,
     Solves balanced entropic OT on the cost ``-scores`` (``sinkhorn``, no gradient), then
     takes each token's top_k experts under the plan. The gates are differentiable in the
     scores with the column potential held fixed. mask (T,) bool: tokens that are padding
-    go nowhere. scores float32, bfloat16 or float16; the solve runs in float32.
+    go nowhere. scores float32, bfloat16 or float16; the solve runs in float32 and waits
+    for its iteration count, as ``sinkhorn`` does.
     """
     if not isinstance(scores, Tensor):
         raise TypeError("scores must be a torch.Tensor")
