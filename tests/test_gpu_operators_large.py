@@ -47,6 +47,33 @@ def test_logits_beyond_2_31_elements():
     assert ((d[at].double() - g).abs() <= 2.0 ** -8 * g.abs() + 500 * U32 * lp.exp()).all()
 
 
+def test_short_rows_beyond_2_31_elements():
+    _need(24)
+    skb = _skb()
+    N, E, k = 35_000_000, 64, 2
+    C = torch.empty(1, N, E, device="cuda", dtype=torch.bfloat16)
+    torch.manual_seed(3)
+    for i in range(0, N, 5_000_000):
+        C[0, i:i + 5_000_000].normal_()
+    g = torch.randn(1, E, device="cuda")
+    C.requires_grad_()
+    r = skb.row_logprobs(C, g, 0.5, top_k=k)
+    d, = torch.autograd.grad(r.entropy, C, torch.ones(1, N, device="cuda"))
+    at = torch.tensor([0, 1, 2 ** 25 - 1, 2 ** 25, 2 ** 25 + 1, N - 1]).cuda()
+    x = (g[0] - C.detach()[0, at].float()).double()
+    lp = torch.log_softmax(2 * x, 1)
+    p = lp.exp()
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(r.top_index[0, at], order)
+    # |z| is below 2 * 12: (2 * 24 + 4) u a term, 8 terms a lane and 3 joins
+    bound = 100 * U32 * 24
+    assert (r.top_logprob.detach()[0, at] - lp.gather(1, order)).abs().max() < bound
+    h = -(p * lp).sum(1)
+    assert (r.entropy.detach()[0, at] - h).abs().max() < bound
+    want = 2 * p * (lp + h[:, None])
+    assert ((d[0, at].double() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * bound * p).all()
+
+
 def test_rows_beyond_2_31_elements():
     _need(22)
     skb = _skb()
@@ -147,3 +174,33 @@ def test_two_captured_graphs_share_nothing():
         torch.cuda.synchronize()
         for a, b in zip(want, outs):
             assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_a_chain_of_dependent_launches_gives_the_same_every_time():
+    # sort, copy, two products and sum start beside the end of the kernel before; two inputs
+    # in turn in one buffer, so that work on stale rows shows
+    skb = _skb()
+    gen = torch.Generator("cuda").manual_seed(5)
+    T, k, D, E = 3001, 2, 256, 16
+    xs = [torch.randn(T, D, device="cuda", generator=gen).bfloat16() for _ in range(2)]
+    ids = [torch.randint(0, E, (T, k), device="cuda", generator=gen) for _ in range(2)]
+    w1 = torch.randn(E, D, 264, device="cuda", generator=gen).bfloat16() / 16
+    w2 = torch.randn(E, 264, D, device="cuda", generator=gen).bfloat16() / 16
+    gates = torch.rand(T, k, device="cuda", generator=gen)
+
+    def chain(x, index):
+        d = skb.expert_dispatch(index, E)
+        y = skb.grouped_matmul(skb.dispatch_rows(x, d), w1, d.offsets)
+        return skb.combine_rows(skb.grouped_matmul(y, w2, d.offsets), d, gates)
+
+    want = []
+    for i in range(2):
+        want.append(chain(xs[i], ids[i]))
+        torch.cuda.synchronize()
+    x, index = xs[0].clone(), ids[0].clone()
+    bad = torch.zeros((), device="cuda")
+    for n in range(200):
+        x.copy_(xs[n % 2])
+        index.copy_(ids[n % 2])
+        bad += (chain(x, index) != want[n % 2]).any()
+    assert bad.item() == 0
