@@ -571,8 +571,9 @@ size_t sk_row_logprobs_backward_workspace_bytes(int64_t B, int64_t N, int64_t M)
  * Gradients of sk_row_logprobs: dX (dense (B,N,M), type of X) and dg (fp32
  * (B,M)), either may be NULL. grad_* are fp32 and may be NULL each; `stats`,
  * `entropy` and `top_index` are the forward's. Empty rows, targets that are
- * not given, out of range or without probability and absent alternatives pass
- * nothing. dg is summed over the rows in a fixed order.
+ * not given, out of range or without probability, absent alternatives and rows
+ * whose upstream gradients are all zero pass nothing, whatever X holds there.
+ * dg is summed over the rows in a fixed order.
  */
 int sk_row_logprobs_backward(const void* X, int dtype, int64_t B, int64_t N, int64_t M,
                              int64_t sXb, int64_t sXn, int64_t sXm, const float* g,

@@ -1424,10 +1424,15 @@ __device__ __forceinline__ uint4 pack16(const float2* x, const float*) {
 }
 
 // dX_v = p_v (c - h lp2) + at [v = target], lp2 = log2 p_v = (x_v - m) k2 - l2;
-// every factor has sign / eps in it already.
+// every factor has sign / eps in it already. l2 = inf marks a row that passes nothing:
+// an empty one, or one whose upstream gradients are all zero. Such a row may hold
+// anything (what mask_a leaves out, positions without a token): -inf takes its values'
+// place, so that p is 0 and no factor meets a NaN.
 struct RowConst {
     float m, l2, c, h, at;
     int target;
+
+    __device__ __forceinline__ bool silent() const { return l2 == INFINITY; }
 };
 
 // COLS: the column sums are wanted; a thread then keeps its columns over all
@@ -1478,10 +1483,8 @@ __global__ void __launch_bounds__(kBwdThreads, 4) k_row_probs_bwd(const RowProbB
                 q.at = q.h = q.c = 0.f;
                 q.m = st.x;
                 q.l2 = st.y * kLog2e;
-                if (st.x == kNegInf && st.y == 0.f) {
-                    q.m = 0.f;  // an empty row: log p = -inf everywhere
-                    q.l2 = INFINITY;
-                } else {
+                bool asked = false;  // of a row that is not empty
+                if (st.x != kNegInf || st.y != 0.f) {
                     if (A.g_lp) {
                         const int64_t t = A.targets[row];
                         bool given = t >= 0 && t < A.M;
@@ -1497,19 +1500,28 @@ __global__ void __launch_bounds__(kBwdThreads, 4) k_row_probs_bwd(const RowProbB
                         }
                     }
                     if (A.g_lse) q.c = A.g_lse[row];
+                    asked = q.at != 0.f || q.c != 0.f;
                     if (A.g_ent) {
                         q.h = A.g_ent[row];
+                        asked = asked || q.h != 0.f;
                         q.c -= q.h * A.entropy[row];
                     }
                     float t = q.at;
                     if (TOP)
 #pragma unroll 4
                         for (int j = 0; j < A.top_k; ++j)
-                            if (A.top_idx[row * A.top_k + j] >= 0)
-                                t += A.g_top[row * A.top_k + j];
+                            if (A.top_idx[row * A.top_k + j] >= 0) {
+                                const float gt = A.g_top[row * A.top_k + j];
+                                asked = asked || gt != 0.f;
+                                t += gt;
+                            }
                     q.c = (q.c - t) * ks;
                     q.h *= ks * kLn2;
                     q.at *= ks;
+                }
+                if (!asked) {
+                    q.m = q.c = q.h = q.at = 0.f;
+                    q.l2 = INFINITY;
                 }
                 rc[r] = q;
             }
@@ -1546,6 +1558,10 @@ __global__ void __launch_bounds__(kBwdThreads, 4) k_row_probs_bwd(const RowProbB
                     }
                 }
                 if (VEC && r + ty < nr) load(X + x_step);
+                if (q.silent()) {
+#pragma unroll
+                    for (int e = 0; e < U * V2; ++e) x[e] = make_float2(kNegInf, kNegInf);
+                }
                 const float2 nm = make_float2(-q.m, -q.m), kk = make_float2(k2, k2);
                 const float2 nl = make_float2(-q.l2, -q.l2), cc = make_float2(q.c, q.c);
                 const float2 nh = make_float2(-q.h, -q.h);
@@ -1557,7 +1573,8 @@ __global__ void __launch_bounds__(kBwdThreads, 4) k_row_probs_bwd(const RowProbB
                 };
                 if (!COLS && VEC && blockIdx.x == 0 && cx < (int)lead && D) {
                     // the columns before the row's first vector, one to a thread
-                    const float v = shaped<SHAPE>(widen(X[cx]), rs, cx);
+                    const float v =
+                        q.silent() ? kNegInf : shaped<SHAPE>(widen(X[cx]), rs, cx);
                     float d = slope(make_float2(v, v)).x + (cx == q.target ? q.at : 0.f);
                     if (TOP)
                         for (int t = 0; t < A.top_k; ++t)

@@ -114,8 +114,9 @@ def row_logprobs(C: Tensor, g: Tensor | None = None, epsilon: float = 0.1,
     Rows with ``mask_a`` False, and rows without a column left, are empty; columns with
     ``mask_b`` False have no probability and their C is not looked at (it may be NaN).
     The best columns are those of largest ``g_j - C_ij`` rounded to fp32. Empty rows,
-    targets not given, out of range or without probability, and absent alternatives pass
-    no gradient. All arithmetic is fp32; the gradient of C is rounded once to C's type.
+    targets not given, out of range or without probability, absent alternatives and rows
+    whose upstream gradients are all zero pass no gradient, whatever such rows hold. All
+    arithmetic is fp32; the gradient of C is rounded once to C's type.
     For the distribution of a column over the rows pass ``C.transpose(1, 2)`` and f.
     """
     if not isinstance(C, Tensor):

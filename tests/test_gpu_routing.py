@@ -115,3 +115,26 @@ def test_layer_step_twice_is_the_same():
 
     for a, b in zip(step(), step()):
         assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_padding_tokens_hold_reaches_nothing(bad):
+    skb = _skb()
+    gen = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=gen)
+    scores, x = r(60, 8), r(60, 32).bfloat16()
+    w1, w2 = (r(8, 32, 48) / 6).bfloat16(), (r(8, 48, 32) / 7).bfloat16()
+    mask = torch.ones(60, dtype=torch.bool)
+    mask[11], mask[50:] = False, False
+    got = []
+    for fill in (0.0, bad):
+        s, y = scores.clone(), x.clone()
+        s[~mask], y[~mask] = fill, fill
+        leaves = [v.cuda().requires_grad_() for v in (y, s, w1, w2)]
+        out, route = skb.sinkhorn_experts(*leaves, top_k=2, epsilon=0.2, mask=mask.cuda())
+        got.append([out.detach(), route.gates.detach(), route.index,
+                    *torch.autograd.grad(out.float().square().sum() + route.rows.entropy.sum(),
+                                         leaves)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.isfinite(b).all()
+    assert all((v[~mask.cuda()] == 0).all() for v in (got[1][0], got[1][3], got[1][4]))

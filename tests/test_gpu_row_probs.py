@@ -441,3 +441,72 @@ def test_same_result_twice_and_under_capture_on_another_stream():
     torch.cuda.synchronize()
     for v, w in zip(step(*leaves(2.0)), out):
         assert torch.equal(v, w)
+
+
+@pytest.mark.parametrize("bad", [math.nan, -math.inf, math.inf])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("B,N,M,k", [(2, 9, 5, 2), (1, 70, 64, 2), (2, 33, 203, 4), (1, 20, 512, 0),
+                                     (2, 6, 1031, 5), (1, 5, 9001, 3)])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_what_a_masked_row_holds_reaches_no_gradient(B, N, M, k, dtype, bad, masked, aligned):
+    """The same bits as with zeros in the rows that mask_a leaves out, and zeros there."""
+    C, g, t, ma, mb = make(B, N, M, TYPES[dtype], M + k)
+    ma[:, 1], ma[:, 0] = False, True
+    mb[:, 0] = True
+    gen = torch.Generator().manual_seed(3)
+    ups = [torch.randn(s, generator=gen).cuda() for s in ((B, N),) * 3 + ((B, N, k),)]
+    got = []
+    for fill in (0.0, bad):
+        Y = C.masked_fill(~ma[..., None], fill)
+        X = Y.cuda() if aligned else torch.nn.functional.pad(Y, (1, 2)).cuda()[..., 1:M + 1]
+        X, G = X.detach().requires_grad_(), g.cuda().requires_grad_()
+        r = _skb().row_logprobs(X, G, 0.5, t.cuda(), k, ma.cuda(), mb.cuda() if masked else None)
+        outs = (r.lse, r.logprob, r.entropy) + ((r.top_logprob,) if k else ())
+        both = torch.autograd.grad(outs, (X, G), ups[:len(outs)], retain_graph=True)
+        alone, = torch.autograd.grad(outs, (G,), ups[:len(outs)])
+        # without dg the rows' vectors start elsewhere
+        r = _skb().row_logprobs(X, g.cuda(), 0.5, t.cuda(), k, ma.cuda(),
+                                mb.cuda() if masked else None)
+        outs = (r.lse, r.logprob, r.entropy) + ((r.top_logprob,) if k else ())
+        got.append([v.detach() for v in outs]
+                   + [*both, alone, *torch.autograd.grad(outs, (X,), ups[:len(outs)])])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    for d in (got[1][len(outs)], got[1][-1]):
+        assert torch.isfinite(d).all() and (d.cpu()[~ma] == 0).all() and (d.cpu()[ma] != 0).any()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V", [40, 333, 3001, 70000])
+def test_rows_that_nothing_is_asked_of_pass_nothing(V, dtype):
+    """Positions without a token whose logits are garbage, as behind the end of a padded
+    batch: no gradient, and the same bits elsewhere."""
+    x = torch.randn(7, V, generator=torch.Generator().manual_seed(V)).to(TYPES[dtype])
+    t = torch.tensor([3, -100, 1, -1, 2, -100, 0])
+    none = t < 0
+    y = x.clone()
+    y[1], y[3], y[5, V // 2] = math.nan, math.inf, math.nan
+    got = []
+    for v in (x, y):
+        X = v.cuda().requires_grad_()
+        r = _skb().token_logprobs(X, t.cuda(), 3)
+        up = torch.where(none, 0.0, 0.5).cuda()
+        d1, = torch.autograd.grad(r.logprob.sum(), X, retain_graph=True)
+        d2, = torch.autograd.grad((r.logprob, r.entropy, r.lse, r.top_logprob), X,
+                                  (torch.ones_like(up), up, up, up[:, None].expand(7, 3)))
+        got.append((r.logprob.detach(), d1, d2))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert all((d[none] == 0).all() and (d[~none] != 0).any() for d in got[1][1:])
+
+
+def test_rows_whose_alternatives_cancel_still_pass_their_gradients():
+    x = torch.randn(2, 50, generator=torch.Generator().manual_seed(6))
+    X = x.cuda().requires_grad_()
+    r = _skb().token_logprobs(X, top_k=2)
+    d, = torch.autograd.grad(r.top_logprob, X, torch.tensor([[1.0, -1.0], [0.0, 0.0]]).cuda())
+    want = torch.zeros(2, 50)
+    i = x[0].topk(2).indices
+    want[0, i[0]], want[0, i[1]] = 1.0, -1.0
+    assert torch.equal(d.cpu(), want)
