@@ -1219,15 +1219,17 @@ __global__ void __launch_bounds__(stream_warps<SHAPE>() * 32, 1) k_row_stream(co
 
 constexpr int64_t kStagedMax = 16384;  // columns of g that are held in shared memory
 
-// Shared memory of a kernel that holds an item's g beside its own: `held` is 0
-// where g is not staged.
+// Let a kernel have `most` bytes of dynamic shared memory where a launch takes more
+// than any kernel may. The limit is one value for all threads of the process: it is
+// the kernel's largest, whatever this launch takes, so that no call lowers another's.
 template <typename K>
-int allow_smem(K kernel, size_t bytes) {
+int allow_smem(K kernel, size_t bytes, size_t most) {
     if (bytes > 16384)
         SK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)bytes));
+                                     (int)most));
     return SK_OK;
 }
+constexpr size_t kStagedBytes = kStagedMax * sizeof(float);
 
 template <typename T, int SHAPE, bool TOP, int U>
 int launch_held(RowProbArgs A, int per_cta, cudaStream_t s) {
@@ -1268,7 +1270,7 @@ int launch_cta(const RowProbArgs& A, int cluster, cudaStream_t s) {
     cfg.blockDim = dim3(32 * kRowWarps);
     cfg.dynamicSmemBytes = A.staged ? align16((int)A.M * 4) : 0;
     cfg.stream = s;
-    const int rc = allow_smem(k_row_cta<T, SHAPE, TOP>, cfg.dynamicSmemBytes);
+    const int rc = allow_smem(k_row_cta<T, SHAPE, TOP>, cfg.dynamicSmemBytes, kStagedBytes);
     if (rc != SK_OK) return rc;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1284,8 +1286,11 @@ int launch_cta(const RowProbArgs& A, int cluster, cudaStream_t s) {
 template <typename T, int SHAPE, bool TOP, int TEAM>
 int launch_stream(const RowProbArgs& A, cudaStream_t s) {
     constexpr int warps = stream_warps<SHAPE>(), teams = warps / TEAM;
-    const size_t smem = (A.staged ? align16((int)A.M * 4) : 0) + (size_t)warps * kAheadBytes;
-    const int rc = allow_smem(k_row_stream<T, SHAPE, TOP, TEAM>, smem);
+    constexpr size_t ahead = (size_t)warps * kAheadBytes, most = kStagedBytes + ahead;
+    static_assert(most + teams * sizeof(RowShared<TOP, TEAM>) + warps * 8 <= 232448,
+                  "shared memory of one CTA");
+    const size_t smem = (A.staged ? align16((int)A.M * 4) : 0) + ahead;
+    const int rc = allow_smem(k_row_stream<T, SHAPE, TOP, TEAM>, smem, most);
     if (rc != SK_OK) return rc;
     const int64_t rows = A.B * A.N;
     const unsigned grid = (unsigned)std::min<int64_t>(148, (rows + teams - 1) / teams);

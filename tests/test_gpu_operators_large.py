@@ -204,3 +204,44 @@ def test_a_chain_of_dependent_launches_gives_the_same_every_time():
         index.copy_(ids[n % 2])
         bad += (chain(x, index) != want[n % 2]).any()
     assert bad.item() == 0
+
+
+def test_two_threads_with_rows_of_different_lengths():
+    """A call keeps its shared memory whatever another thread launches meanwhile (the entry
+    points themselves: between two calls of the wrappers the threads seldom meet)."""
+    import threading
+    from sinkhorn_b200 import _lib
+    skb, L = _skb(), _lib.load()
+    codes, begin = [], threading.Barrier(4)
+
+    def prepared(M, top_k, N):
+        C = torch.randn(2, N, M, device="cuda")
+        g = torch.randn(2, M, device="cuda")
+        want = skb.row_logprobs(C, g, 0.5, top_k=top_k)
+        lse, ent = torch.empty(2, N, device="cuda"), torch.empty(2, N, device="cuda")
+        lp = torch.empty(2, N, max(top_k, 1), device="cuda")
+        idx = torch.empty(2, N, max(top_k, 1), device="cuda", dtype=torch.int64)
+        stream = torch.cuda.Stream()
+        args = (C.data_ptr(), 0, 2, N, M, N * M, M, 1, g.data_ptr(), 0.5, 1, None, None, None,
+                top_k, lse.data_ptr(), None, ent.data_ptr(), lp.data_ptr() if top_k else None,
+                idx.data_ptr() if top_k else None, None, None, 0, stream.cuda_stream)
+        return args, lse, want, (C, g, ent, lp, idx, stream)
+
+    # rows that take a CTA each, and rows that are streamed
+    work = [prepared(M, k, N) for M, k, N in ((16384, 0, 5), (5000, 0, 5), (16384, 2, 300),
+                                              (4100, 2, 300))]
+    torch.cuda.synchronize()
+
+    def run(args):
+        begin.wait()
+        codes.append({L.sk_row_logprobs(*args) for _ in range(4000)})
+
+    threads = [threading.Thread(target=run, args=(w[0],)) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [{0}] * 4
+    for _, lse, want, _ in work:
+        assert torch.equal(lse, want.lse)
