@@ -603,8 +603,10 @@ int sk_expert_dispatch(const int64_t* index, int64_t slots, int experts, int* or
 /*
  * rows[position[t,j]] = x[t] for the k slots of each of T tokens; rows (T k, D)
  * dense, zero behind offsets[experts]. x has row stride ldx (elements) and
- * unit column stride. A position outside 0..T k - 1 counts as dropped, here
- * and below.
+ * unit column stride. A position outside 0..n - 1, n = min(offsets[experts],
+ * T k), counts as dropped, here and below. No two positions may be equal, and
+ * places before n that no position names are left as they are: where a plan
+ * was edited, the calls with `order` below.
  */
 int sk_dispatch_rows(const void* x, int dtype, int64_t T, int k, int64_t D, int64_t ldx,
                      const int* position, const int* offsets, int experts, void* rows,
@@ -629,6 +631,23 @@ int sk_combine_rows_backward(const void* grad_out, const void* y, int dtype, int
                              int64_t D, int64_t ldg, int64_t ldy, const int* position,
                              const int* offsets, int experts, const float* weights, void* grad_y,
                              float* grad_weights, void* stream);
+
+/*
+ * The same three for any plan: slot s holds place p = position[s] where
+ * order[p] = s too and p < offsets[experts]; other slots count as dropped, and
+ * all places that no slot holds are zero in `rows` and grad_y.
+ */
+int sk_dispatch_plan_rows(const void* x, int dtype, int64_t T, int k, int64_t D, int64_t ldx,
+                          const int* order, const int* position, const int* offsets,
+                          int experts, void* rows, void* stream);
+int sk_combine_plan_rows(const void* y, int dtype, int64_t T, int k, int64_t D, int64_t ldy,
+                         const int* order, const int* position, const int* offsets, int experts,
+                         const float* weights, void* out, void* stream);
+int sk_combine_plan_rows_backward(const void* grad_out, const void* y, int dtype, int64_t T,
+                                  int k, int64_t D, int64_t ldg, int64_t ldy, const int* order,
+                                  const int* position, const int* offsets, int experts,
+                                  const float* weights, void* grad_y, float* grad_weights,
+                                  void* stream);
 
 /*
  * dst[g][r][0..ld) = src[g * sg + r * sr + 0..width) of 16-bit elements, ld =

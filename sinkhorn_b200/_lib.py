@@ -118,6 +118,12 @@ SIGNATURES = {
     "sk_combine_rows": (_INT, [_P, _INT, _I64, _INT, _I64, _I64, _P, _P, _INT, _P, _P, _P]),
     "sk_combine_rows_backward": (_INT, [_P, _P, _INT, _I64, _INT, _I64, _I64, _I64, _P, _P,
                                         _INT, _P, _P, _P, _P]),
+    "sk_dispatch_plan_rows": (_INT, [_P, _INT, _I64, _INT, _I64, _I64, _P, _P, _P, _INT, _P,
+                                     _P]),
+    "sk_combine_plan_rows": (_INT, [_P, _INT, _I64, _INT, _I64, _I64, _P, _P, _P, _INT, _P, _P,
+                                    _P]),
+    "sk_combine_plan_rows_backward": (_INT, [_P, _P, _INT, _I64, _INT, _I64, _I64, _I64, _P, _P,
+                                             _P, _INT, _P, _P, _P, _P]),
     "sk_grouped_pack": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P]),
     "sk_grouped_matmul": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64,
                                  _P, _P, _P]),

@@ -191,6 +191,7 @@ struct RowsArgs {
     int64_t T;
     int k;
     int words;
+    const int* order;  // the slot at each place, or NULL: positions alone count
     const int* position;
     const int* offsets;  // its last entry: rows that are held
     int E;
@@ -201,20 +202,44 @@ struct RowsArgs {
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;  // most words of a row to a lane at once
 
-// The slot's place; one that is no row of the T k (a plan not made by
-// sk_expert_dispatch) counts as dropped.
-__device__ __forceinline__ int place_of(const RowsArgs& A, int64_t t, int j) {
-    const int p = __ldg(A.position + t * A.k + j);
-    return p < A.T * A.k ? p : -1;
+// Places that can be held: those before the last offset.
+__device__ __forceinline__ int places(const RowsArgs& A) {
+    return (int)min((int64_t)max(A.offsets[A.E], 0), A.T * A.k);
+}
+
+// The slot's place p of n, -1 where it has none. A slot holds its place where the place
+// names it, too: of a plan that was edited (slots dropped for an expert over its
+// capacity, two slots at one place) each row has one writer then, and rows without one
+// are known to the place alone (gap_at).
+__device__ __forceinline__ int named_place(const RowsArgs& A, int n, int64_t slot) {
+    const int p = __ldg(A.position + slot);
+    return (unsigned)p < (unsigned)n ? p : -1;
+}
+__device__ __forceinline__ bool holds(const RowsArgs& A, int64_t slot, int p) {
+    return !A.order || __ldg(A.order + p) == (int)slot;
+}
+__device__ __forceinline__ bool gap_at(const RowsArgs& A, int64_t p) {
+    const int s = __ldg(A.order + p);
+    return s < 0 || s >= A.T * A.k || __ldg(A.position + s) != (int)p;
 }
 
 template <int W>
-__device__ __forceinline__ void zero_rows_behind(const RowsArgs& A, int64_t gw, int64_t nw,
-                                                 int lane) {
+__device__ __forceinline__ void zero_row(const RowsArgs& A, int64_t p, int lane) {
     using Word = typename WordOf<W>::type;
-    for (int64_t p = max(A.offsets[A.E], 0) + gw; p < A.T * A.k; p += nw) {
-        Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
-        for (int c = lane; c < A.words; c += 32) o[c] = Word{};
+    Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
+    for (int c = lane; c < A.words; c += 32) o[c] = Word{};
+}
+
+// Rows that no slot writes: those behind the last group, and gaps before it (looked for
+// by the last warps first, which have the least to copy).
+template <int W>
+__device__ __forceinline__ void zero_unheld(const RowsArgs& A, int n, int64_t gw, int64_t nw,
+                                            int lane) {
+    for (int64_t p = n + gw; p < A.T * A.k; p += nw) zero_row<W>(A, p, lane);
+    if (!A.order) return;
+    for (int64_t p0 = (nw - 1 - gw) * 32; p0 < n; p0 += nw * 32) {
+        unsigned gaps = __ballot_sync(0xffffffffu, p0 + lane < n && gap_at(A, p0 + lane));
+        for (; gaps; gaps &= gaps - 1) zero_row<W>(A, p0 + __ffs(gaps) - 1, lane);
     }
 }
 
@@ -226,6 +251,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_dispatch_rows(const RowsArgs A
     const int lane = threadIdx.x & 31;
     const int64_t gw = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) >> 5;
     const int64_t nw = (int64_t)gridDim.x * (kCopyThreads / 32);
+    const int held = places(A);
     for (int64_t t = gw; t < A.T; t += nw) {
         const Word* const x = reinterpret_cast<const Word*>(A.x) + t * A.ldx;
         for (int c = lane; c < A.words; c += 32 * kCopyUnroll) {
@@ -234,8 +260,8 @@ __global__ void __launch_bounds__(kCopyThreads) k_dispatch_rows(const RowsArgs A
             for (int u = 0; u < kCopyUnroll; ++u)
                 if (c + u * 32 < A.words) v[u] = x[c + u * 32];
             for (int j = 0; j < A.k; ++j) {
-                const int p = place_of(A, t, j);
-                if (p < 0) continue;
+                const int p = named_place(A, held, t * A.k + j);
+                if (p < 0 || !holds(A, t * A.k + j, p)) continue;
                 Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
 #pragma unroll
                 for (int u = 0; u < kCopyUnroll; ++u)
@@ -243,7 +269,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_dispatch_rows(const RowsArgs A
             }
         }
     }
-    zero_rows_behind<W>(A, gw, nw, lane);
+    zero_unheld<W>(A, held, gw, nw, lane);
 }
 
 // ox[t] = sum_j w[t,j] y[position[t,j]], in fp32, rounded once.
@@ -256,6 +282,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_combine_rows(const RowsArgs A)
     const int lane = threadIdx.x & 31;
     const int64_t gw = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) >> 5;
     const int64_t nw = (int64_t)gridDim.x * (kCopyThreads / 32);
+    const int held = places(A);
     for (int64_t t = gw; t < A.T; t += nw) {
         Word* const o = reinterpret_cast<Word*>(A.ox) + t * A.ldox;
         for (int c = lane; c < A.words; c += 32 * U) {
@@ -265,14 +292,16 @@ __global__ void __launch_bounds__(kCopyThreads) k_combine_rows(const RowsArgs A)
 #pragma unroll
                 for (int i = 0; i < n; ++i) sum[u][i] = 0.f;
             for (int j = 0; j < A.k; ++j) {
-                const int p = place_of(A, t, j);
+                const int p = named_place(A, held, t * A.k + j);
                 if (p < 0) continue;
+                const bool own = holds(A, t * A.k + j, p);  // (on its way beside the row)
                 const float w = A.w ? __ldg(A.w + t * A.k + j) : 1.f;
                 const Word* const y = reinterpret_cast<const Word*>(A.y) + p * A.ldy;
                 Elems<T, W> v[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (c + u * 32 < A.words) v[u].word = y[c + u * 32];
+                if (!own) continue;
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (c + u * 32 < A.words)
@@ -303,12 +332,14 @@ __global__ void __launch_bounds__(kCopyThreads) k_combine_rows_bwd(const RowsArg
     const int lane = threadIdx.x & 31;
     const int64_t gw = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) >> 5;
     const int64_t nw = (int64_t)gridDim.x * (kCopyThreads / 32);
+    const int held = places(A);
     for (int64_t t = gw; t < A.T; t += nw) {
         const Word* const x = reinterpret_cast<const Word*>(A.x) + t * A.ldx;
         for (int j = 0; j < A.k; ++j) {
-            const int p = place_of(A, t, j);
+            const int p = named_place(A, held, t * A.k + j);
             float dot = 0.f;
             if (p >= 0) {
+                const bool own = holds(A, t * A.k + j, p);  // (on its way beside the rows)
                 const float w = A.w ? __ldg(A.w + t * A.k + j) : 1.f;
                 const Word* const y = reinterpret_cast<const Word*>(A.y) + p * A.ldy;
                 Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
@@ -327,13 +358,14 @@ __global__ void __launch_bounds__(kCopyThreads) k_combine_rows_bwd(const RowsArg
 #pragma unroll
                                 for (int i = 0; i < n; ++i)
                                     dot = fmaf(d[u].get(i), v[u].get(i), dot);
-                            if (A.oy) {
+                            if (A.oy && own) {
 #pragma unroll
                                 for (int i = 0; i < n; ++i) d[u].set(i, w * d[u].get(i));
                                 o[c + u * 32] = d[u].word;
                             }
                         }
                 }
+                if (!own) dot = 0.f;
             }
             if (A.dw) {
                 dot = warp_sum(dot);
@@ -341,7 +373,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_combine_rows_bwd(const RowsArg
             }
         }
     }
-    if (A.oy) zero_rows_behind<W>(A, gw, nw, lane);
+    if (A.oy) zero_unheld<W>(A, held, gw, nw, lane);
 }
 
 unsigned rows_grid(int64_t T) {
@@ -425,6 +457,85 @@ int run_combine_typed(RowsArgs A, int dtype, int64_t D, bool bwd, cudaStream_t s
     return run_combine_wide<__half>(A, w, bwd, s);
 }
 
+int dispatch_rows(const void* x, int dtype, int64_t T, int k, int64_t D, int64_t ldx,
+                  const int* order, const int* position, const int* offsets, int experts,
+                  void* rows, cudaStream_t s) {
+    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
+    if (rc != SK_OK) return rc;
+    if (!x || !rows) return fail(SK_ERR_ARG, "x or rows is NULL");
+    if (ldx < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
+    const int elem = dtype == SK_FP32 ? 4 : 2;
+    const int w = word_bytes(D, elem, {x, rows}, {ldx, D});
+    if (w < elem) return fail(SK_ERR_LAYOUT, "rows are not aligned to their elements");
+    RowsArgs A{};
+    A.x = x;
+    A.oy = rows;
+    A.ldx = ldx * elem / w;
+    A.ldoy = D * elem / w;
+    A.T = T;
+    A.k = k;
+    A.words = (int)(D * elem / w);
+    A.order = order;
+    A.position = position;
+    A.offsets = offsets;
+    A.E = experts;
+    if (w == 16) return run_dispatch<16>(A, s);
+    if (w == 8) return run_dispatch<8>(A, s);
+    if (w == 4) return run_dispatch<4>(A, s);
+    return run_dispatch<2>(A, s);
+}
+
+int combine_rows(const void* y, int dtype, int64_t T, int k, int64_t D, int64_t ldy,
+                 const int* order, const int* position, const int* offsets, int experts,
+                 const float* weights, void* out, cudaStream_t s) {
+    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
+    if (rc != SK_OK) return rc;
+    if (!y || !out) return fail(SK_ERR_ARG, "y or out is NULL");
+    if (ldy < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
+    RowsArgs A{};
+    A.y = y;
+    A.ox = out;
+    A.ldy = ldy;
+    A.ldox = D;
+    A.T = T;
+    A.k = k;
+    A.order = order;
+    A.position = position;
+    A.offsets = offsets;
+    A.E = experts;
+    A.w = weights;
+    return run_combine_typed(A, dtype, D, false, s);
+}
+
+int combine_rows_backward(const void* grad_out, const void* y, int dtype, int64_t T, int k,
+                          int64_t D, int64_t ldg, int64_t ldy, const int* order,
+                          const int* position, const int* offsets, int experts,
+                          const float* weights, void* grad_y, float* grad_weights,
+                          cudaStream_t s) {
+    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
+    if (rc != SK_OK) return rc;
+    if (!grad_out) return fail(SK_ERR_ARG, "grad_out is NULL");
+    if (!grad_y && !grad_weights) return fail(SK_ERR_ARG, "no gradient is asked for");
+    if (grad_weights && !y) return fail(SK_ERR_ARG, "grad_weights needs y");
+    if (ldg < 0 || ldy < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
+    RowsArgs A{};
+    A.x = grad_out;
+    A.y = y;
+    A.oy = grad_y;
+    A.ldx = ldg;
+    A.ldy = ldy;
+    A.ldoy = D;
+    A.T = T;
+    A.k = k;
+    A.order = order;
+    A.position = position;
+    A.offsets = offsets;
+    A.E = experts;
+    A.w = weights;
+    A.dw = grad_weights;
+    return run_combine_typed(A, dtype, D, true, s);
+}
+
 int64_t sort_tiles(int64_t S) { return (S + kSortTile - 1) / kSortTile; }
 
 }  // namespace
@@ -467,83 +578,57 @@ int sk_expert_dispatch(const int64_t* index, int64_t slots, int experts, int* or
 int sk_dispatch_rows(const void* x, int dtype, int64_t T, int k, int64_t D, int64_t ldx,
                      const int* position, const int* offsets, int experts, void* rows,
                      void* stream) {
-    using namespace sk;
-    clear_error();
-    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
-    if (rc != SK_OK) return rc;
-    if (!x || !rows) return fail(SK_ERR_ARG, "x or rows is NULL");
-    if (ldx < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
-    const int elem = dtype == SK_FP32 ? 4 : 2;
-    const int w = word_bytes(D, elem, {x, rows}, {ldx, D});
-    if (w < elem) return fail(SK_ERR_LAYOUT, "rows are not aligned to their elements");
-    RowsArgs A{};
-    A.x = x;
-    A.oy = rows;
-    A.ldx = ldx * elem / w;
-    A.ldoy = D * elem / w;
-    A.T = T;
-    A.k = k;
-    A.words = (int)(D * elem / w);
-    A.position = position;
-    A.offsets = offsets;
-    A.E = experts;
-    cudaStream_t s = (cudaStream_t)stream;
-    if (w == 16) return run_dispatch<16>(A, s);
-    if (w == 8) return run_dispatch<8>(A, s);
-    if (w == 4) return run_dispatch<4>(A, s);
-    return run_dispatch<2>(A, s);
+    sk::clear_error();
+    return sk::dispatch_rows(x, dtype, T, k, D, ldx, nullptr, position, offsets, experts, rows,
+                             (cudaStream_t)stream);
+}
+
+int sk_dispatch_plan_rows(const void* x, int dtype, int64_t T, int k, int64_t D, int64_t ldx,
+                          const int* order, const int* position, const int* offsets,
+                          int experts, void* rows, void* stream) {
+    sk::clear_error();
+    if (!order) return sk::fail(SK_ERR_ARG, "order is NULL");
+    return sk::dispatch_rows(x, dtype, T, k, D, ldx, order, position, offsets, experts, rows,
+                             (cudaStream_t)stream);
 }
 
 int sk_combine_rows(const void* y, int dtype, int64_t T, int k, int64_t D, int64_t ldy,
                     const int* position, const int* offsets, int experts, const float* weights,
                     void* out, void* stream) {
-    using namespace sk;
-    clear_error();
-    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
-    if (rc != SK_OK) return rc;
-    if (!y || !out) return fail(SK_ERR_ARG, "y or out is NULL");
-    if (ldy < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
-    RowsArgs A{};
-    A.y = y;
-    A.ox = out;
-    A.ldy = ldy;
-    A.ldox = D;
-    A.T = T;
-    A.k = k;
-    A.position = position;
-    A.offsets = offsets;
-    A.E = experts;
-    A.w = weights;
-    return run_combine_typed(A, dtype, D, false, (cudaStream_t)stream);
+    sk::clear_error();
+    return sk::combine_rows(y, dtype, T, k, D, ldy, nullptr, position, offsets, experts, weights,
+                            out, (cudaStream_t)stream);
+}
+
+int sk_combine_plan_rows(const void* y, int dtype, int64_t T, int k, int64_t D, int64_t ldy,
+                         const int* order, const int* position, const int* offsets, int experts,
+                         const float* weights, void* out, void* stream) {
+    sk::clear_error();
+    if (!order) return sk::fail(SK_ERR_ARG, "order is NULL");
+    return sk::combine_rows(y, dtype, T, k, D, ldy, order, position, offsets, experts, weights,
+                            out, (cudaStream_t)stream);
 }
 
 int sk_combine_rows_backward(const void* grad_out, const void* y, int dtype, int64_t T, int k,
                              int64_t D, int64_t ldg, int64_t ldy, const int* position,
                              const int* offsets, int experts, const float* weights, void* grad_y,
                              float* grad_weights, void* stream) {
-    using namespace sk;
-    clear_error();
-    const int rc = check_rows_args(dtype, T, k, D, experts, position, offsets);
-    if (rc != SK_OK) return rc;
-    if (!grad_out) return fail(SK_ERR_ARG, "grad_out is NULL");
-    if (!grad_y && !grad_weights) return fail(SK_ERR_ARG, "no gradient is asked for");
-    if (grad_weights && !y) return fail(SK_ERR_ARG, "grad_weights needs y");
-    if (ldg < 0 || ldy < 0) return fail(SK_ERR_LAYOUT, "negative row stride");
-    RowsArgs A{};
-    A.x = grad_out;
-    A.y = y;
-    A.oy = grad_y;
-    A.ldx = ldg;
-    A.ldy = ldy;
-    A.ldoy = D;
-    A.T = T;
-    A.k = k;
-    A.position = position;
-    A.offsets = offsets;
-    A.E = experts;
-    A.w = weights;
-    A.dw = grad_weights;
-    return run_combine_typed(A, dtype, D, true, (cudaStream_t)stream);
+    sk::clear_error();
+    return sk::combine_rows_backward(grad_out, y, dtype, T, k, D, ldg, ldy, nullptr, position,
+                                     offsets, experts, weights, grad_y, grad_weights,
+                                     (cudaStream_t)stream);
+}
+
+int sk_combine_plan_rows_backward(const void* grad_out, const void* y, int dtype, int64_t T,
+                                  int k, int64_t D, int64_t ldg, int64_t ldy, const int* order,
+                                  const int* position, const int* offsets, int experts,
+                                  const float* weights, void* grad_y, float* grad_weights,
+                                  void* stream) {
+    sk::clear_error();
+    if (!order) return sk::fail(SK_ERR_ARG, "order is NULL");
+    return sk::combine_rows_backward(grad_out, y, dtype, T, k, D, ldg, ldy, order, position,
+                                     offsets, experts, weights, grad_y, grad_weights,
+                                     (cudaStream_t)stream);
 }
 
 }  // extern "C"

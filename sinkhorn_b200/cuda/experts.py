@@ -35,24 +35,25 @@ def unit_rows(x: Tensor) -> Tensor:
     return x if x.stride(1) == 1 or x.shape[1] == 1 and x.is_contiguous() else x.contiguous()
 
 
-def gather_rows(x: Tensor, position: Tensor, offsets: Tensor) -> Tensor:
-    """sk_dispatch_rows: rows (T k, D) of x (T, D)."""
+def gather_rows(x: Tensor, order: Tensor, position: Tensor, offsets: Tensor) -> Tensor:
+    """sk_dispatch_plan_rows: rows (T k, D) of x (T, D)."""
     x = unit_rows(x)
     t, k = position.shape
     D = x.shape[1]
     rows = torch.empty(t * k, D, device=x.device, dtype=x.dtype)
     if rows.numel():
         with T.on(x.device):
-            rc = T.lib().sk_dispatch_rows(
-                x.data_ptr(), T.DTYPES[x.dtype], t, k, D, x.stride(0), position.data_ptr(),
-                offsets.data_ptr(), offsets.numel() - 1, rows.data_ptr(),
+            rc = T.lib().sk_dispatch_plan_rows(
+                x.data_ptr(), T.DTYPES[x.dtype], t, k, D, x.stride(0), order.data_ptr(),
+                position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1, rows.data_ptr(),
                 T.stream_of(x.device))
-            T.check(rc, "sk_dispatch_rows")
+            T.check(rc, "sk_dispatch_plan_rows")
     return rows
 
 
-def sum_rows(y: Tensor, position: Tensor, offsets: Tensor, weights: Tensor | None) -> Tensor:
-    """sk_combine_rows: (T, D) from y (T k, D); weights dense float32 (T, k) or None."""
+def sum_rows(y: Tensor, order: Tensor, position: Tensor, offsets: Tensor,
+             weights: Tensor | None) -> Tensor:
+    """sk_combine_plan_rows: (T, D) from y (T k, D); weights dense float32 (T, k) or None."""
     y = unit_rows(y)
     t, k = position.shape
     D = y.shape[1]
@@ -62,17 +63,17 @@ def sum_rows(y: Tensor, position: Tensor, offsets: Tensor, weights: Tensor | Non
     if not k:
         return out.zero_()
     with T.on(y.device):
-        rc = T.lib().sk_combine_rows(
-            y.data_ptr(), T.DTYPES[y.dtype], t, k, D, y.stride(0), position.data_ptr(),
-            offsets.data_ptr(), offsets.numel() - 1, T.ptr(weights), out.data_ptr(),
-            T.stream_of(y.device))
-        T.check(rc, "sk_combine_rows")
+        rc = T.lib().sk_combine_plan_rows(
+            y.data_ptr(), T.DTYPES[y.dtype], t, k, D, y.stride(0), order.data_ptr(),
+            position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1, T.ptr(weights),
+            out.data_ptr(), T.stream_of(y.device))
+        T.check(rc, "sk_combine_plan_rows")
     return out
 
 
-def sum_rows_backward(grad: Tensor, y: Tensor, position: Tensor, offsets: Tensor,
-                      weights: Tensor | None, need_y: bool, need_w: bool):
-    """sk_combine_rows_backward: (grad_y, grad_weights); unneeded ones are None."""
+def sum_rows_backward(grad: Tensor, y: Tensor, order: Tensor, position: Tensor,
+                      offsets: Tensor, weights: Tensor | None, need_y: bool, need_w: bool):
+    """sk_combine_plan_rows_backward: (grad_y, grad_weights); unneeded ones are None."""
     t, k = position.shape
     D = y.shape[1]
     grad = unit_rows(grad)
@@ -84,11 +85,11 @@ def sum_rows_backward(grad: Tensor, y: Tensor, position: Tensor, offsets: Tensor
     if not D:
         return dy, None if dw is None else dw.zero_()
     with T.on(y.device):
-        rc = T.lib().sk_combine_rows_backward(
+        rc = T.lib().sk_combine_plan_rows_backward(
             grad.data_ptr(), y.data_ptr(), T.DTYPES[y.dtype], t, k, D, grad.stride(0),
-            y.stride(0), position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
-            T.ptr(weights), T.ptr(dy), T.ptr(dw), T.stream_of(y.device))
-        T.check(rc, "sk_combine_rows_backward")
+            y.stride(0), order.data_ptr(), position.data_ptr(), offsets.data_ptr(),
+            offsets.numel() - 1, T.ptr(weights), T.ptr(dy), T.ptr(dw), T.stream_of(y.device))
+        T.check(rc, "sk_combine_plan_rows_backward")
     return dy, dw
 
 

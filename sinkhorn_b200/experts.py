@@ -26,7 +26,12 @@ MAX_EXPERTS = 1024
 
 @dataclass
 class ExpertDispatch:
-    """Where each slot (token t's j-th choice, number t * k + j) goes. int32 tensors."""
+    """Where each slot (token t's j-th choice, number t * k + j) goes. int32 tensors.
+
+    A slot holds place ``position[t, j]`` where ``order`` names the slot there and the place
+    lies before the last offset; any other slot counts as dropped, and a place that no slot
+    holds is a row of zeros. So a plan may be edited, as for experts over their capacity:
+    -1 in ``position`` drops a slot."""
 
     order: Tensor
     """(T k,) the slot at each place, -1 behind the last group"""
@@ -90,45 +95,45 @@ def _check_rows(x: Tensor, name: str, rows: int) -> None:
 
 class DispatchRowsFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, x: Tensor, position: Tensor, offsets: Tensor) -> Tensor:
-        ctx.save_for_backward(position, offsets)
-        return gather_rows(x, position, offsets)
+    def forward(ctx: Any, x: Tensor, order: Tensor, position: Tensor,
+                offsets: Tensor) -> Tensor:
+        ctx.save_for_backward(order, position, offsets)
+        return gather_rows(x, order, position, offsets)
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: Tensor):
-        position, offsets = ctx.saved_tensors
-        return sum_rows(grad, position, offsets, None), None, None
+        return sum_rows(grad, *ctx.saved_tensors, None), None, None, None
 
 
 class CombineRowsFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, y: Tensor, weights: Tensor | None, position: Tensor,
+    def forward(ctx: Any, y: Tensor, weights: Tensor | None, order: Tensor, position: Tensor,
                 offsets: Tensor) -> Tensor:
-        ctx.save_for_backward(y, weights, position, offsets)
-        return sum_rows(y, position, offsets, T.floats(weights))
+        ctx.save_for_backward(y, weights, order, position, offsets)
+        return sum_rows(y, order, position, offsets, T.floats(weights))
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: Tensor):
-        y, weights, position, offsets = ctx.saved_tensors
-        dy, dw = sum_rows_backward(grad, y, position, offsets, T.floats(weights),
+        y, weights, order, position, offsets = ctx.saved_tensors
+        dy, dw = sum_rows_backward(grad, y, order, position, offsets, T.floats(weights),
                                    ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return dy, None if dw is None else dw.to(weights.dtype), None, None
+        return dy, None if dw is None else dw.to(weights.dtype), None, None, None
 
 
 def dispatch_rows(x: Tensor, dispatch: ExpertDispatch) -> Tensor:
     """Rows of x (T, D) in expert order: (T k, D), row ``position[t, j]`` is x[t].
 
-    Rows behind the last group are zero. float32, bfloat16 or float16; rows may be
+    Rows that no slot holds are zero, those behind the last group among them. float32, bfloat16 or float16; rows may be
     strided. The gradient of x[t] is the sum over its rows, in fp32, rounded once.
     """
     T.check_cuda(x, "x")
     _check_dispatch(dispatch, x.device)
     _check_rows(x, "x", dispatch.position.shape[0])
     if not T.needs_grad(x):
-        return gather_rows(x, dispatch.position, dispatch.offsets)
-    return DispatchRowsFunction.apply(x, dispatch.position, dispatch.offsets)
+        return gather_rows(x, dispatch.order, dispatch.position, dispatch.offsets)
+    return DispatchRowsFunction.apply(x, dispatch.order, dispatch.position, dispatch.offsets)
 
 
 def combine_rows(y: Tensor, dispatch: ExpertDispatch, weights: Tensor | None = None) -> Tensor:
@@ -152,8 +157,10 @@ def combine_rows(y: Tensor, dispatch: ExpertDispatch, weights: Tensor | None = N
         if weights.device != y.device:
             raise ValueError(f"weights are on {weights.device}, y is on {y.device}")
     if not T.needs_grad(y, weights):
-        return sum_rows(y, dispatch.position, dispatch.offsets, T.floats(weights))
-    return CombineRowsFunction.apply(y, weights, dispatch.position, dispatch.offsets)
+        return sum_rows(y, dispatch.order, dispatch.position, dispatch.offsets,
+                        T.floats(weights))
+    return CombineRowsFunction.apply(y, weights, dispatch.order, dispatch.position,
+                                     dispatch.offsets)
 
 
 class GroupedMatmulFunction(torch.autograd.Function):

@@ -190,3 +190,126 @@ def test_captured_and_replayed_on_another_stream():
     order, position, _ = plan(index.cpu(), 16)
     assert torch.equal(d.order.cpu(), order)
     assert torch.equal(out.cpu(), x.cpu() * (position >= 0).sum(1, keepdim=True))
+
+
+def held_by(d):
+    """place -> slot of a plan: slot s holds place p where position[s] = p, order[p] = s and p
+    lies before the last offset."""
+    order, position = d.order.tolist(), d.position.reshape(-1).tolist()
+    n = min(len(order), int(d.offsets[-1]))
+    return {p: s for s, p in enumerate(position) if 0 <= p < n and order[p] == s}
+
+
+def _edit(d, how):
+    if how == "places dropped":
+        d.position[1, 0], d.position[7, 1], d.position[20, 0] = -1, -1, 10 ** 6
+    elif how == "order dropped":
+        d.order[3], d.order[17] = -1, 2 ** 30
+    elif how == "two slots at one place":
+        d.position[4, 0], d.position[9, 1] = d.position[5, 1], d.position[6, 0]
+    elif how == "fewer rows":
+        d.offsets[-1] -= 9
+    elif how == "more rows":
+        d.offsets[-1] = 10 ** 6
+    elif how == "places exchanged":  # in both: a plan as good as before
+        a, b = int(d.position[2, 0]), int(d.position[12, 1])
+        d.position[2, 0], d.position[12, 1] = b, a
+        d.order[a], d.order[b] = 12 * 2 + 1, 2 * 2
+
+
+@pytest.mark.parametrize("how", ["places dropped", "order dropped", "two slots at one place",
+                                 "fewer rows", "more rows", "places exchanged"])
+@pytest.mark.parametrize("dtype,D", [("fp32", 64), ("fp32", 130), ("fp32", 33), ("bf16", 1000),
+                                     ("bf16", 36), ("fp16", 34), ("fp16", 77)])
+def test_places_that_no_slot_holds_are_zero(how, dtype, D):
+    """Plans that a caller has edited, as for experts over their capacity: nothing that the
+    memory held before shows."""
+    skb, dt = _skb(), TYPES[dtype]
+    T, k, E = 40, 2, 5
+    gen = torch.Generator().manual_seed(D)
+    d = skb.expert_dispatch(torch.randint(0, E, (T, k), generator=gen).cuda(), E)
+    _edit(d, how)
+    held = held_by(d)
+    x = torch.randn(T, D, generator=gen).to(dt)
+    y = torch.randn(T * k, D, generator=gen).to(dt)
+    w, up = torch.rand(T, k, generator=gen), torch.randn(T, D, generator=gen).to(dt)
+
+    def stale():  # what torch.empty gives next
+        keep = [torch.full((T * k, D), float("nan"), device="cuda", dtype=dt) for _ in range(4)]
+        del keep
+
+    stale()
+    rows = skb.dispatch_rows(x.cuda(), d)
+    want = torch.zeros(T * k, D, dtype=dt)
+    for p, s in held.items():
+        want[p] = x[s // k]
+    assert torch.equal(rows.cpu(), want)
+
+    Y, W = y.cuda().requires_grad_(), w.cuda().requires_grad_()
+    out = skb.combine_rows(Y, d, W)
+    stale()
+    dy, dw = torch.autograd.grad(out, (Y, W), up.cuda())
+    wout, wdy = torch.zeros(T, D, dtype=torch.float64), torch.zeros(T * k, D, dtype=torch.float64)
+    wdw, size = torch.zeros(T * k, dtype=torch.float64), torch.zeros(T * k, dtype=torch.float64)
+    terms = torch.zeros(T, D, dtype=torch.float64)
+    for p, s in held.items():
+        a = w.reshape(-1)[s].double()
+        wout[s // k] += a * y[p].double()
+        terms[s // k] += (a * y[p].double()).abs()
+        wdy[p] = a * up[s // k].double()
+        wdw[s] = (up[s // k].double() * y[p].double()).sum()
+        size[s] = (up[s // k].double() * y[p].double()).abs().sum()
+    half, tiny = torch.finfo(dt).eps / 2, torch.finfo(dt).tiny
+    assert ((out.detach().double().cpu() - wout).abs() <= half * wout.abs() + k * U32 * terms
+            + tiny).all()
+    assert ((dy.double().cpu() - wdy).abs() <= (half + U32) * wdy.abs() + tiny).all()
+    # a lane adds up to D / 32 products, the warp five sums
+    assert ((dw.double().cpu().reshape(-1) - wdw).abs() <= (D / 32 + 8) * U32 * size).all()
+    # the gradient of dispatch_rows is combine_rows of the same plan
+    X = x.cuda().requires_grad_()
+    dx, = torch.autograd.grad(skb.dispatch_rows(X, d), X, y.cuda())
+    assert torch.equal(dx, skb.combine_rows(y.cuda(), d))
+
+
+def test_products_of_a_plan_with_dropped_places():
+    skb = _skb()
+    gen = torch.Generator().manual_seed(1)
+    d = skb.expert_dispatch(torch.randint(0, 3, (50, 2), generator=gen).cuda(), 3)
+    d.position[10:20] = -1
+    x = torch.randn(50, 64, generator=gen).bfloat16().cuda().requires_grad_()
+    w = (torch.randn(3, 64, 48, generator=gen) / 8).bfloat16().cuda().requires_grad_()
+    junk = [torch.full((100, n), float("nan"), device="cuda", dtype=torch.bfloat16)
+            for n in (64, 48) * 3]
+    del junk
+    out = skb.combine_rows(skb.grouped_matmul(skb.dispatch_rows(x, d), w, d.offsets), d)
+    dx, dw = torch.autograd.grad(out.float().sum(), (x, w))
+    for v in (out, dx):
+        assert torch.isfinite(v).all() and (v[10:20] == 0).all() and (v[:10] != 0).any()
+    for e in range(3):  # every row of dW_e's columns is the sum of the expert's held rows
+        held = [s // 2 for s in d.order[int(d.offsets[e]):int(d.offsets[e + 1])].tolist()
+                if not 10 <= s // 2 < 20]
+        rows = x.detach().cpu()[held].double()
+        # the sum of n values, in fp32, rounded once
+        bound = 2.0 ** -8 * rows.sum(0).abs() + 2 * len(held) * U32 * rows.abs().sum(0)
+        assert ((dw[e].double().cpu() - rows.sum(0)[:, None]).abs() <= bound[:, None]).all()
+
+
+def test_entry_points_without_the_order_agree_on_plans_of_the_sort():
+    from sinkhorn_b200 import _lib
+    skb, L = _skb(), _lib.load()
+    T, k, E, D = 60, 2, 5, 72
+    d = skb.expert_dispatch(choices(T, k, E, 8).cuda(), E)
+    x, w = torch.randn(T, D, device="cuda"), torch.rand(T, k, device="cuda")
+    y = torch.randn(T * k, D, device="cuda").requires_grad_()
+    out = skb.combine_rows(y, d, w.requires_grad_())
+    dy, dw = torch.autograd.grad(out, (y, w), x)
+    new = lambda *s: torch.full(s, float("nan"), device="cuda")
+    rows, sums, gy, gw = new(T * k, D), new(T, D), new(T * k, D), new(T, k)
+    s, p = torch.cuda.current_stream().cuda_stream, (d.position.data_ptr(), d.offsets.data_ptr())
+    ptr = lambda t: t.data_ptr()
+    assert L.sk_dispatch_rows(ptr(x), 0, T, k, D, D, *p, E, ptr(rows), s) == 0
+    assert L.sk_combine_rows(ptr(y), 0, T, k, D, D, *p, E, ptr(w), ptr(sums), s) == 0
+    assert L.sk_combine_rows_backward(ptr(x), ptr(y), 0, T, k, D, D, D, *p, E, ptr(w), ptr(gy),
+                                      ptr(gw), s) == 0
+    assert torch.equal(rows, skb.dispatch_rows(x, d)) and torch.equal(sums, out)
+    assert torch.equal(gy, dy) and torch.equal(gw, dw)

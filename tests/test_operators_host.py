@@ -265,3 +265,16 @@ def test_public_names():
                  "sinkhorn_route", "sinkhorn_experts", "Route"):
         assert hasattr(skb, name) and name in skb.__all__
     assert hasattr(skb.SinkhornOutput, "assign")
+
+
+@pytest.mark.parametrize("call", [
+    lambda L, o, p: L.sk_dispatch_plan_rows(_P, 1, 4, 2, 8, 8, o, p, _P, 2, _P, None),
+    lambda L, o, p: L.sk_combine_plan_rows(_P, 1, 4, 2, 8, 8, o, p, _P, 2, None, _P, None),
+    lambda L, o, p: L.sk_combine_plan_rows_backward(_P, _P, 1, 4, 2, 8, 8, 8, o, p, _P, 2, None,
+                                                    _P, None, None),
+], ids=["dispatch", "combine", "backward"])
+def test_calls_with_a_plan_need_its_order_and_positions(call):
+    from sinkhorn_b200 import _lib
+    lib = _lib.load()
+    for order, position in ((None, _P), (_P, None)):
+        assert call(lib, order, position) == ARG and lib.sk_last_error().decode()
