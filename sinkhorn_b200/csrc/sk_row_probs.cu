@@ -1329,8 +1329,8 @@ int launch_rows_sized(const RowProbArgs& A, cudaStream_t s) {
     }
     const bool runs = (SHAPE == kPlain || A.N >= 64) && rows < INT_MAX / 2;
     if (bytes <= 16384 && rows >= 148 * 16 && runs) return launch_stream<T, SHAPE, TOP, 1>(A, s);
-    if (SHAPE != kPlain && bytes > 8192 && rows >= 148 * 4 && runs)
-        return launch_stream<T, SHAPE, TOP, 4>(A, s);
+    if constexpr (SHAPE != kPlain)
+        if (bytes > 8192 && rows >= 148 * 4 && runs) return launch_stream<T, SHAPE, TOP, 4>(A, s);
     int cluster = 1;
     while (cluster < 8 && rows * cluster * 2 <= 148 * 4 &&
            bytes > (int64_t)cluster * kRowWarps * 32 * 4 * 16)

@@ -510,3 +510,38 @@ def test_rows_whose_alternatives_cancel_still_pass_their_gradients():
     i = x[0].topk(2).indices
     want[0, i[0]], want[0, i[1]] = 1.0, -1.0
     assert torch.equal(d.cpu(), want)
+
+
+def _on_host(ref):
+    return {name: v.cpu() for name, v in ref.items()}
+
+
+@pytest.mark.parametrize("dtype,V", [("fp32", 515), ("fp32", 1999), ("fp32", 4091), ("bf16", 1999),
+                                     ("bf16", 4096), ("bf16", 8190), ("fp16", 1031),
+                                     ("fp16", 8190)])
+@pytest.mark.parametrize("k", [0, 3, 20])
+def test_many_rows_of_logits(dtype, V, k):
+    """Rows that are streamed without a potential, on 16 bytes and off it."""
+    T = 2500
+    base = 3 * torch.randn(T, V + 3, generator=torch.Generator().manual_seed(V + k))
+    base = base.to(TYPES[dtype]).cuda()
+    t = torch.randint(-1, V, (T,), generator=torch.Generator().manual_seed(k))
+    for x in (base[:, :V].contiguous(), base[:, 1:V + 1]):
+        r = _skb().token_logprobs(x, t.cuda(), k, temperature=0.7)
+        check(r, _on_host(plain(x.double(), 1 / 0.7, t.cuda(), k)), V, k)
+
+
+@pytest.mark.parametrize("dtype,B,N,M", [
+    ("fp32", 5, 701, 700), ("fp32", 5, 701, 4091), ("bf16", 5, 701, 1999), ("fp16", 5, 701, 8190),
+    ("fp32", 5, 701, 5003), ("bf16", 5, 701, 9001), ("fp16", 7, 97, 8500),  # four warps a row
+    ("fp32", 3, 257, 16500), ("bf16", 3, 257, 17001),                        # g not staged
+])
+@pytest.mark.parametrize("k", [0, 3, 20])
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_rows_of_several_items(dtype, B, N, M, k, masked):
+    """A CTA's run of rows crosses items, each with its own g and masks."""
+    C, g, t, ma, mb = (v.cuda() for v in make(B, N, M, TYPES[dtype], M + k))
+    if not masked:
+        ma = mb = None
+    r = _skb().row_logprobs(C, g, 0.25, t, k, ma, mb)
+    check(r, _on_host(plain(shaped(C, g, ma, mb), 4.0, t.reshape(-1), k)), M, k)
