@@ -192,3 +192,16 @@ def test_int64_offsets_captured_and_replayed_with_other_lengths():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, _gmm(x, w, offsets))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("S,K,N,ends,transposed", [
+    (2700, 264, 2100, [0, 2300, 2600], False),   # rows: nine column tiles, nine rows of tiles
+    (2700, 520, 328, [5, 100, 2700], True),
+    (300, 2100, 520, [0, 130, 290], False),      # weights: nine column tiles, three rows
+    (300, 520, 2100, [0, 130, 290], True),
+    (4700, 264, 264, [0, 4500, 4700], False),    # two bands and a half
+])
+def test_tiles_in_several_bands(S, K, N, ends, transposed, dtype):
+    x, w = make(S, 2, K, N, dtype, S + K)
+    check(x, w.transpose(1, 2).contiguous().transpose(1, 2) if transposed else w, ends)
