@@ -28,7 +28,12 @@ namespace {
 
 constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortTile = 2048;  // slots of a CTA
+constexpr int kSortTile = 2048;  // slots of a CTA at once
+// Every CTA of the second launch adds up the counts of all, so there are at most two
+// to an SM: more slots are more tiles of a CTA's run, one after the other, and the work
+// grows with the slots and not with their square (8M slots, 256 experts: 1324 us with a
+// tile to each CTA, 209 us so; 65536 slots take a tile each in both).
+constexpr int kSortCtas = 2 * 148;
 constexpr int kMaxExperts = 1024;
 
 __device__ __forceinline__ int expert_of(const int64_t* index, int64_t s, int64_t S, int E) {
@@ -37,29 +42,32 @@ __device__ __forceinline__ int expert_of(const int64_t* index, int64_t s, int64_
     return e >= 0 && e < E ? (int)e : -1;
 }
 
-// hist[tile][e]: the tile's slots of each expert.
+// hist[run][e]: the slots of each expert in a CTA's run of `run` slots.
 __global__ void __launch_bounds__(kSortThreads) k_expert_count(const int64_t* index, int64_t S,
-                                                              int E, int* hist) {
+                                                              int64_t run, int E, int* hist) {
     __shared__ int count[kMaxExperts];
     pdl_wait();
     pdl_trigger();
     for (int e = threadIdx.x; e < E; e += kSortThreads) count[e] = 0;
     __syncthreads();
-    const int64_t s0 = (int64_t)blockIdx.x * kSortTile;
+    const int64_t end = min(S, (blockIdx.x + 1) * run);
+    for (int64_t s0 = blockIdx.x * run; s0 < end; s0 += kSortTile) {
 #pragma unroll
-    for (int i = 0; i < kSortTile / kSortThreads; ++i) {
-        const int e = expert_of(index, s0 + i * kSortThreads + threadIdx.x, S, E);
-        if (e >= 0) atomicAdd(&count[e], 1);  // counts only: their order is no matter
+        for (int i = 0; i < kSortTile / kSortThreads; ++i) {
+            const int e = expert_of(index, s0 + i * kSortThreads + threadIdx.x, S, E);
+            if (e >= 0) atomicAdd(&count[e], 1);  // counts only: their order is no matter
+        }
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += kSortThreads)
         hist[(int64_t)blockIdx.x * E + e] = count[e];
 }
 
-// Places of the tile's slots. A warp takes a run of consecutive slots, 32 at a
-// time; lanes of one expert rank themselves by match.any.
+// Places of the slots of a CTA's run, tile by tile. A warp takes consecutive slots of a
+// tile, 32 at a time; lanes of one expert rank themselves by match.any.
 __global__ void __launch_bounds__(kSortThreads) k_expert_place(const int64_t* index, int64_t S,
-                                                              int E, int tiles, const int* hist,
+                                                              int64_t run, int E,
+                                                              const int* hist,
                                                               int* order, int* position,
                                                               int* offsets) {
     extern __shared__ int sm[];
@@ -68,42 +76,70 @@ __global__ void __launch_bounds__(kSortThreads) k_expert_place(const int64_t* in
     __shared__ int wsum[kSortWarps];
     __shared__ int carry;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t s0 =
-        (int64_t)blockIdx.x * kSortTile + warp * (kSortTile / kSortWarps);
+    const int64_t end = min(S, (blockIdx.x + 1) * run);
+    int64_t tile = blockIdx.x * run;
     constexpr int R = kSortTile / kSortThreads;
     int e[R];
+    auto slot = [&](int i) {
+        return tile + warp * (kSortTile / kSortWarps) + i * 32 + lane;
+    };
+    // the warp's slots of each expert
+    auto count = [&] {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+            if (e[i] >= 0 && lane == __ffs(same) - 1) wcount[warp * E + e[i]] += __popc(same);
+            __syncwarp();
+        }
+    };
+    // the earlier warps' counts in place of each one's; their sum
+    auto sum_warps = [&](int x) {
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+            const int c = wcount[w * E + x];
+            wcount[w * E + x] = sum;
+            sum += c;
+        }
+        return sum;
+    };
+    // every slot of the tile to its place; each warp's counts are added to the earlier ones
+    auto place = [&] {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const unsigned same = __match_any_sync(0xffffffffu, e[i]);
+            const int64_t s = slot(i);
+            int at = -1;
+            if (e[i] >= 0) {
+                at = start[e[i]] + wcount[warp * E + e[i]] + __popc(same & ((1u << lane) - 1u));
+                if (at < S) order[at] = (int)s;
+            }
+            if (s < S) position[s] = at;
+            __syncwarp();
+            if (e[i] >= 0 && lane == __ffs(same) - 1) wcount[warp * E + e[i]] += __popc(same);
+            __syncwarp();
+        }
+    };
     for (int i = threadIdx.x; i < kSortWarps * E; i += kSortThreads) wcount[i] = 0;
     if (threadIdx.x == 0) carry = 0;
     pdl_wait();
     pdl_trigger();
 #pragma unroll
-    for (int i = 0; i < R; ++i) e[i] = expert_of(index, s0 + i * 32 + lane, S, E);
+    for (int i = 0; i < R; ++i) e[i] = expert_of(index, slot(i), S, E);
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const unsigned same = __match_any_sync(0xffffffffu, e[i]);
-        if (e[i] >= 0 && lane == __ffs(same) - 1) wcount[warp * E + e[i]] += __popc(same);
-        __syncwarp();
-    }
+    count();
     __syncthreads();
-    // Per expert: the earlier warps' counts, the earlier tiles', and the total,
+    // Per expert: the earlier warps' counts, the earlier CTAs', and the total,
     // whose running sum over the experts gives the offsets.
     for (int base = 0; base < E; base += kSortThreads) {
         const int x = base + threadIdx.x;
         int total = 0, before = 0;
         if (x < E) {
-            int run = 0;
-#pragma unroll
-            for (int w = 0; w < kSortWarps; ++w) {
-                const int c = wcount[w * E + x];
-                wcount[w * E + x] = run;
-                run += c;
-            }
-            if (tiles == 1) {
-                total = run;
-            } else {
+            total = sum_warps(x);  // (a single CTA has a single tile)
+            if (gridDim.x > 1) {
+                total = 0;
 #pragma unroll 8
-                for (int t = 0; t < tiles; ++t) {
+                for (int t = 0; t < (int)gridDim.x; ++t) {
                     const int c = hist[(int64_t)t * E + x];
                     if (t < (int)blockIdx.x) before += c;
                     total += c;
@@ -130,19 +166,22 @@ __global__ void __launch_bounds__(kSortThreads) k_expert_place(const int64_t* in
     }
     const int held = carry;
     if (blockIdx.x == 0 && threadIdx.x == 0) offsets[E] = held;
+    place();
+    for (tile += kSortTile; tile < end; tile += kSortTile) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const unsigned same = __match_any_sync(0xffffffffu, e[i]);
-        const int64_t s = s0 + i * 32 + lane;
-        int at = -1;
-        if (e[i] >= 0) {
-            at = start[e[i]] + wcount[warp * E + e[i]] + __popc(same & ((1u << lane) - 1u));
-            if (at < S) order[at] = (int)s;
+        for (int i = 0; i < R; ++i) e[i] = expert_of(index, slot(i), S, E);
+        __syncthreads();  // the last tile is placed: its last warp's counts are its sums
+        for (int x = threadIdx.x; x < E; x += kSortThreads) {
+            start[x] += wcount[(kSortWarps - 1) * E + x];
+#pragma unroll
+            for (int w = 0; w < kSortWarps; ++w) wcount[w * E + x] = 0;
         }
-        if (s < S) position[s] = at;
-        __syncwarp();
-        if (e[i] >= 0 && lane == __ffs(same) - 1) wcount[warp * E + e[i]] += __popc(same);
-        __syncwarp();
+        __syncthreads();
+        count();
+        __syncthreads();
+        for (int x = threadIdx.x; x < E; x += kSortThreads) sum_warps(x);
+        __syncthreads();
+        place();
     }
     // places behind the last group
     for (int64_t p = held + (int64_t)blockIdx.x * kSortThreads + threadIdx.x; p < S;
@@ -536,7 +575,15 @@ int combine_rows_backward(const void* grad_out, const void* y, int dtype, int64_
     return run_combine_typed(A, dtype, D, true, s);
 }
 
-int64_t sort_tiles(int64_t S) { return (S + kSortTile - 1) / kSortTile; }
+// Slots of a CTA's run: whole tiles, one where there are few.
+int64_t sort_run(int64_t S) {
+    const int64_t tiles = (S + kSortTile - 1) / kSortTile;
+    return (tiles + kSortCtas - 1) / kSortCtas * kSortTile;
+}
+int sort_ctas(int64_t S) {
+    const int64_t run = sort_run(S);
+    return (int)((S + run - 1) / run);
+}
 
 }  // namespace
 }  // namespace sk
@@ -545,7 +592,7 @@ extern "C" {
 
 size_t sk_expert_dispatch_workspace_bytes(int64_t slots, int experts) {
     if (slots <= sk::kSortTile || experts <= 0) return 0;  // one CTA counts for itself
-    return sk::align_up(sizeof(int) * (size_t)sk::sort_tiles(slots) * experts);
+    return sk::align_up(sizeof(int) * (size_t)sk::sort_ctas(slots) * experts);
 }
 
 int sk_expert_dispatch(const int64_t* index, int64_t slots, int experts, int* order,
@@ -562,15 +609,16 @@ int sk_expert_dispatch(const int64_t* index, int64_t slots, int experts, int* or
     if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4 != 0))
         return fail(SK_ERR_WORKSPACE, "workspace too small for sk_expert_dispatch");
     cudaStream_t s = (cudaStream_t)stream;
-    const int tiles = (int)sort_tiles(slots);
-    if (tiles > 1) {
-        launch_pdl(k_expert_count, dim3(tiles), dim3(kSortThreads), 0, s, index, slots, experts,
-                   (int*)workspace);
+    const int ctas = sort_ctas(slots);
+    const int64_t run = sort_run(slots);
+    if (ctas > 1) {
+        launch_pdl(k_expert_count, dim3(ctas), dim3(kSortThreads), 0, s, index, slots, run,
+                   experts, (int*)workspace);
         SK_LAUNCHED("k_expert_count");
     }
     const size_t smem = sizeof(int) * (size_t)experts * (1 + kSortWarps);
-    launch_pdl(k_expert_place, dim3(tiles), dim3(kSortThreads), smem, s, index, slots, experts,
-               tiles, (const int*)workspace, order, position, offsets);
+    launch_pdl(k_expert_place, dim3(ctas), dim3(kSortThreads), smem, s, index, slots, run,
+               experts, (const int*)workspace, order, position, offsets);
     SK_LAUNCHED("k_expert_place");
     return SK_OK;
 }

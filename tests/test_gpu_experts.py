@@ -313,3 +313,23 @@ def test_entry_points_without_the_order_agree_on_plans_of_the_sort():
                                       ptr(gw), s) == 0
     assert torch.equal(rows, skb.dispatch_rows(x, d)) and torch.equal(sums, out)
     assert torch.equal(gy, dy) and torch.equal(gw, dw)
+
+
+@pytest.mark.parametrize("T,k,E", [(606209, 1, 300), (700001, 1, 1024), (1500007, 4, 256),
+                                   (5000001, 1, 1), (2600000, 3, 7)])
+def test_sort_of_many_slots(T, k, E):
+    """More slots than one run of 2048 to a CTA."""
+    gen = torch.Generator("cuda").manual_seed(T)
+    index = torch.randint(-1, E + 1, (T, k), device="cuda", generator=gen)
+    d = _skb().expert_dispatch(index, E)
+    flat = index.reshape(-1)
+    key = torch.where((flat >= 0) & (flat < E), flat, E)
+    order = torch.sort(key, stable=True).indices
+    counts = torch.bincount(key, minlength=E + 1)
+    held = int(counts[:E].sum())
+    offsets = torch.cat([counts.new_zeros(1), counts[:E].cumsum(0)])
+    position = torch.full_like(flat, -1)
+    position[order[:held]] = torch.arange(held, device="cuda")
+    assert torch.equal(d.offsets, offsets.int())
+    assert torch.equal(d.order[:held], order[:held].int()) and (d.order[held:] == -1).all()
+    assert torch.equal(d.position.reshape(-1), position.int())

@@ -278,3 +278,14 @@ def test_calls_with_a_plan_need_its_order_and_positions(call):
     lib = _lib.load()
     for order, position in ((None, _P), (_P, None)):
         assert call(lib, order, position) == ARG and lib.sk_last_error().decode()
+
+
+def test_the_sorts_counts_do_not_grow_with_the_slots():
+    """Every CTA of the sort adds up all counts: few, whatever the slots, or its work would
+    grow with their square."""
+    from sinkhorn_b200 import _lib
+    L = _lib.load()
+    for experts in (1, 256, 1024):
+        most = L.sk_expert_dispatch_workspace_bytes(2 ** 31 - 1, experts)
+        assert 0 < most <= 4 * 1024 * experts + 256
+        assert most >= L.sk_expert_dispatch_workspace_bytes(1 << 20, experts)
