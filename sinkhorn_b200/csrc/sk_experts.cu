@@ -14,7 +14,9 @@
 // gradients for 16385 x 4 rows of 1536 50 us and 73 us (5.0 and 6.2 TB/s). The sort is
 // two launches of 6 us and 8 us for 65536 slots, one of 5 us up to 2048.
 // The kernels are launched as programmatic dependents of one another (see
-// sk_common.cuh): sort and copy of 32768 x 2 rows 83 us apart, 76 us so.
+// sk_common.cuh): sort and copy of 32768 x 2 rows 83 us apart, 76 us so. What a kernel
+// before may still be writing when they start is read by plain loads behind pdl_wait():
+// the read-only path is for data that nothing writes while the kernel lives.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -251,15 +253,15 @@ __device__ __forceinline__ int places(const RowsArgs& A) {
 // capacity, two slots at one place) each row has one writer then, and rows without one
 // are known to the place alone (gap_at).
 __device__ __forceinline__ int named_place(const RowsArgs& A, int n, int64_t slot) {
-    const int p = __ldg(A.position + slot);
+    const int p = A.position[slot];
     return (unsigned)p < (unsigned)n ? p : -1;
 }
 __device__ __forceinline__ bool holds(const RowsArgs& A, int64_t slot, int p) {
-    return !A.order || __ldg(A.order + p) == (int)slot;
+    return !A.order || A.order[p] == (int)slot;
 }
 __device__ __forceinline__ bool gap_at(const RowsArgs& A, int64_t p) {
-    const int s = __ldg(A.order + p);
-    return s < 0 || s >= A.T * A.k || __ldg(A.position + s) != (int)p;
+    const int s = A.order[p];
+    return s < 0 || s >= A.T * A.k || A.position[s] != (int)p;
 }
 
 template <int W>
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_combine_rows(const RowsArgs A)
                 const int p = named_place(A, held, t * A.k + j);
                 if (p < 0) continue;
                 const bool own = holds(A, t * A.k + j, p);  // (on its way beside the row)
-                const float w = A.w ? __ldg(A.w + t * A.k + j) : 1.f;
+                const float w = A.w ? A.w[t * A.k + j] : 1.f;
                 const Word* const y = reinterpret_cast<const Word*>(A.y) + p * A.ldy;
                 Elems<T, W> v[U];
 #pragma unroll
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_combine_rows_bwd(const RowsArg
             float dot = 0.f;
             if (p >= 0) {
                 const bool own = holds(A, t * A.k + j, p);  // (on its way beside the rows)
-                const float w = A.w ? __ldg(A.w + t * A.k + j) : 1.f;
+                const float w = A.w ? A.w[t * A.k + j] : 1.f;
                 const Word* const y = reinterpret_cast<const Word*>(A.y) + p * A.ldy;
                 Word* const o = reinterpret_cast<Word*>(A.oy) + p * A.ldoy;
                 for (int c = lane; c < A.words; c += 32 * U) {

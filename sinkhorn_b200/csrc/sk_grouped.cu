@@ -194,7 +194,7 @@ __device__ void plan_groups(const GroupedArgs& A, GroupedShared* sh, int lane) {
     for (int base = 0; base <= A.E + 1; base += 32) {
         // entry i: first row of group i + 1 (offsets[i]; S after the last)
         const int i = base + lane;
-        int o = i <= A.E ? min(max(__ldg(A.offsets + i), 0), A.S) : A.S;
+        int o = i <= A.E ? min(max(A.offsets[i], 0), A.S) : A.S;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, o, s);
