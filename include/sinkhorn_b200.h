@@ -549,7 +549,9 @@ int sk_backward(const float* C, int64_t B, int64_t N, int64_t M, int64_t sCb,
  * top_logprob NaN. Any output may be NULL (logprob exactly when targets is;
  * top_logprob and top_index only when top_k is 0). `stats` (2 floats per row)
  * is what the backward needs. X may have any row strides; its columns have
- * stride 1. The row form of the plan's conditional distribution
+ * stride 1. The call does not wait for its kernel, so a bounded wait that gives up
+ * inside it has no status to return: the statistics and log probabilities of the
+ * rows it touched become NaN. The row form of the plan's conditional distribution
  * (SinkhornOutput.transport_plan normalised by rows, src/sinkhorn/sinkhorn.py:27-54).
  */
 int sk_row_logprobs(const void* X, int dtype, int64_t B, int64_t N, int64_t M, int64_t sXb,
@@ -664,6 +666,9 @@ int sk_grouped_pack(const void* src, int64_t groups, int64_t rows, int64_t width
  * all fp16, sums in fp32, rounded once. Every row of x and W starts on 16 bytes
  * (address and strides; else SK_ERR_LAYOUT: sk_grouped_pack). offsets (E+1) is
  * device memory; entries that fall or leave [0,S] are brought back. E <= 1024.
+ * The call does not wait for its kernel: a bounded wait that gives up inside it
+ * turns the output tiles that it left unfinished into NaN, and the call has
+ * returned SK_OK (SK_ERR_TIMEOUT is the solver's). The same holds for the next one.
  * The gradient of x is the same call on dy with K, N and swk, swn exchanged.
  */
 int sk_grouped_matmul(const void* x, int dtype, int64_t S, int64_t K, int64_t ldx, const void* w,

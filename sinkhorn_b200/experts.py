@@ -193,7 +193,8 @@ def grouped_matmul(x: Tensor, w: Tensor, offsets: Tensor) -> Tensor:
     get zero gradient. Offsets that decrease or leave 0..S are clamped. Sums are in fp32,
     rounded once. Any K and N; rows that do not start on 16 bytes (K or N no multiple of 8)
     are copied once more. w may be stored (E, N, K) and passed transposed; its gradient then
-    has that layout, too. Up to 1024 groups.
+    has that layout, too. Up to 1024 groups. A wait inside the kernel that gives up shows as
+    NaN in the output, not as an error: nothing here waits for the device.
     """
     for name, t, dims in (("x", x, 2), ("w", w, 3)):
         T.check_cuda(t, name)

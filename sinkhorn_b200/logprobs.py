@@ -117,6 +117,7 @@ def row_logprobs(C: Tensor, g: Tensor | None = None, epsilon: float = 0.1,
     targets not given, out of range or without probability, absent alternatives and rows
     whose upstream gradients are all zero pass no gradient, whatever such rows hold. All
     arithmetic is fp32; the gradient of C is rounded once to C's type.
+    A wait inside the kernel that gives up shows as NaN, not as an error.
     For the distribution of a column over the rows pass ``C.transpose(1, 2)`` and f.
     """
     if not isinstance(C, Tensor):
