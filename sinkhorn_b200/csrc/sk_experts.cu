@@ -6,7 +6,7 @@
 // so the result does not depend on how the kernels are scheduled -- and the
 // tokens' rows are copied there (dispatch) and summed back with the gates'
 // weights (combine). Slots whose index is no expert are dropped; the rows
-// behind offsets[E] are zero.
+// that no slot holds, those behind offsets[E] among them, are zero.
 //
 // All three row kernels go by token, one warp each: the token's row is read or
 // written once, its k slots are whole rows elsewhere. They are bound by DRAM: 32768
