@@ -51,8 +51,9 @@ def sinkhorn_route(scores: Tensor, top_k: int = 1, epsilon: float = 0.1,
     Solves balanced entropic OT on the cost ``-scores`` (``sinkhorn``, no gradient), then
     takes each token's top_k experts under the plan. The gates are differentiable in the
     scores with the column potential held fixed. mask (T,) bool: tokens that are padding
-    go nowhere. scores float32, bfloat16 or float16; the solve runs in float32 and waits
-    for its iteration count, as ``sinkhorn`` does.
+    go nowhere, and so does a token without a score above -inf (all of them NaN, too: its
+    ``rows.lse`` says so). scores float32, bfloat16 or float16; the solve runs in float32
+    and waits for its iteration count, as ``sinkhorn`` does.
     """
     if not isinstance(scores, Tensor):
         raise TypeError("scores must be a torch.Tensor")
@@ -79,9 +80,11 @@ def sinkhorn_route(scores: Tensor, top_k: int = 1, epsilon: float = 0.1,
                        threshold=threshold, check_every=check_every)
     rows = row_logprobs(C, out.g, epsilon, top_k=top_k, mask_a=mask)
     index = rows.top_index[0]
-    # (a masked token's are all -inf: bounded, so that 0 * nan stays out of the gradient)
-    p = torch.softmax(rows.top_logprob[0].clamp(min=-1e30), -1)
-    gates = torch.where(index >= 0, p, torch.zeros_like(p))
+    held = index >= 0
+    # (a masked token's are all -inf: replaced, so that 0 * nan stays out of the gradient;
+    # a NaN among the held ones shows in the gates and in the gradient)
+    p = torch.softmax(torch.where(held, rows.top_logprob[0], -1e30), -1)
+    gates = torch.where(held, p, torch.zeros_like(p))
     return Route(index, gates, expert_dispatch(index, E), rows, out.n_iters, out.converged)
 
 

@@ -138,3 +138,21 @@ def test_what_padding_tokens_hold_reaches_nothing(bad):
     for a, b in zip(*got):
         assert torch.equal(a, b) and torch.isfinite(b).all()
     assert all((v[~mask.cuda()] == 0).all() for v in (got[1][0], got[1][3], got[1][4]))
+
+
+def test_a_nan_score_shows_in_its_own_token():
+    skb = _skb()
+    gen = torch.Generator().manual_seed(9)
+    r = lambda *s: torch.randn(*s, generator=gen).cuda()
+    scores, x = r(40, 8), r(40, 16).bfloat16()
+    w1, w2 = r(8, 16, 16).bfloat16(), r(8, 16, 16).bfloat16()
+    scores[3, 2] = float("nan")
+    scores[7] = float("nan")
+    s = scores.requires_grad_()
+    out, route = skb.sinkhorn_experts(x, s, w1, w2, top_k=2)
+    d, = torch.autograd.grad(out.float().sum(), s)
+    others = torch.ones(40, dtype=torch.bool)
+    others[3] = others[7] = False
+    assert out[3].isnan().all() and route.gates[3].isnan().all() and d[3].isnan().any()
+    assert (route.index[7] == -1).all() and route.rows.lse[0, 7].isnan() and (out[7] == 0).all()
+    assert torch.isfinite(out[others]).all() and torch.isfinite(d[others]).all()
