@@ -11,8 +11,9 @@
 // All three row kernels go by token, one warp each: the token's row is read or
 // written once, its k slots are whole rows elsewhere. They are bound by DRAM: 32768
 // x 2 rows of 2048 bf16 64 us (6.3 TB/s, 96% of a copy), and back with their
-// gradients for 16385 x 4 rows of 1536 45 us and 78 us (5.6 and 5.8 TB/s, each called in a row). The sort is
-// two launches of 6 us and 8 us for 65536 slots, one of 5 us up to 2048.
+// gradients for 16385 x 4 rows of 1536 45 us and 78 us (5.6 and 5.8 TB/s, each called in
+// a row). The sort is two launches of 6 us and 8 us for 65536 slots, one of 5 us up to
+// 2048.
 // The kernels are launched as programmatic dependents of one another (see
 // sk_common.cuh): sort and copy of 32768 x 2 rows 83 us apart, 76 us so. What a kernel
 // before may still be writing when they start is read by plain loads behind pdl_wait():
